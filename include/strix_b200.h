@@ -197,6 +197,68 @@ int strix_w8a8_int8_gemm(void* out, int32_t* acc_out, const void* a_q, const flo
                          int64_t a_stride, int64_t w_stride, int64_t out_stride,
                          strix_stream_t stream);
 
+/* FP8 W8A8 GEMM with block scales:
+ *   out[m, n] = sum_b a_scale[m, b] * w_scale[n / 128, b]
+ *                     * (sum_{k in block b} a_q[m, k] * w[n, k])  (+ bias[n])
+ * with blocks of 128 columns. a_q e4m3 [m, k], w e4m3 [n, k] (row strides in
+ * bytes, multiples of 16); a_scale fp32 [m, ceil(k / 128)], w_scale fp32 [ceil(n /
+ * 128), ceil(k / 128)], any element strides; out bf16 / fp16 / fp32 (out_kind 0 / 1
+ * / 2) [m, n]; bias NULL or [n] in the output's type. k must be a multiple of 16
+ * (the last block may be short), m and n are free. Sums and scales in fp32, one
+ * rounding at the end; no scratch, and the result does not depend on timing. The
+ * reference has this weight format with 16-bit activations only
+ * (csrc/gemm/fp8_wmma_gemm.hip, schema csrc/torch_ops.cpp:256). tcgen05
+ * kind::f8f6f4; a launch may follow its predecessor's start (programmatic
+ * dependent launch) but reads nothing before that one has ended. */
+int strix_w8a8_fp8_gemm(void* out, const void* a_q, const float* a_scale, const void* w,
+                        const float* w_scale, const void* bias, int64_t m, int64_t n, int64_t k,
+                        int64_t a_stride, int64_t w_stride, int64_t out_stride, int64_t sa_stride_m,
+                        int64_t sa_stride_k, int64_t sw_stride_n, int64_t sw_stride_k, int out_kind,
+                        strix_stream_t stream);
+
+/* The gate-up product of an MLP that ends in the input form of the down product:
+ * w e4m3 [2 n, k] holds the gate rows and then the up rows, w_scale fp32 [ceil(2 n /
+ * 128), ceil(k / 128)]; with G, U the fp32 sums of strix_w8a8_fp8_gemm over the two
+ * halves, y = act(G) * U (gate_act 1 silu, 2 gelu_tanh) is quantised as
+ * strix_act_mul_quant does: q e4m3 [m, n], scales fp32 [m, ceil(n / 128)]. n and k
+ * multiples of 16. workspace: strix_w8a8_fp8_gated_workspace(m, n, k) bytes on a
+ * 16-byte boundary (0: none needed, NULL allowed), free again when the launches
+ * have ended. Launches that may run at the same time need workspaces of their own. */
+int64_t strix_w8a8_fp8_gated_workspace(int64_t m, int64_t n, int64_t k);
+int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, const float* a_scale, const void* w,
+                         const float* w_scale, void* workspace, int64_t workspace_bytes, int64_t m,
+                         int64_t n, int64_t k, int64_t a_stride, int64_t w_stride, int64_t q_stride,
+                         int64_t s_stride, int64_t sa_stride_m, int64_t sa_stride_k,
+                         int64_t sw_stride_n, int64_t sw_stride_k, int gate_act, strix_stream_t stream);
+
+/* Root-mean-square norm (with the residual's addition) into 8 bits, the step in
+ * front of a W8A8 GEMM:
+ *   s = x + residual (s = x where residual is NULL), fp32
+ *   residual_out = s rounded to x's type (NULL: not stored; may be x or residual
+ *                  itself, with its stride, else apart from both)
+ *   y = s / sqrt(mean(s^2) + eps) * weight
+ * fp8 != 0: q e4m3 [rows, k], scales fp32 [rows, ceil(k / 128)] = amax / 448 of each
+ * (row, 128 columns), k a multiple of 16. fp8 == 0: q int8 [rows, k], scales fp32
+ * [rows] (s_stride apart) = amax / 127, k a multiple of 8. A scale below the smallest
+ * normal number (an all-zero group) is 1; q = y / scale to nearest even; a NaN or an
+ * infinity in a group shows in its scale. x, residual bf16 (fp16 if in_f16), weight
+ * of the same type or fp32 (weight_f32); element strides, rows on 16-byte boundaries,
+ * k at most 65,536. vLLM's norm does this step in the reference's deployment, in
+ * 16 bits; its GEMMs quantise (csrc/gemm/w8a8_wmma_gemm.hip:508-529). */
+int strix_rms_norm_quant(const void* x, const void* residual, void* residual_out, const void* weight,
+                         void* q, float* scales, int64_t rows, int64_t k, int64_t x_stride,
+                         int64_t r_stride, int64_t ro_stride, int64_t q_stride, int64_t s_stride,
+                         float eps, int in_f16, int weight_f32, int fp8, strix_stream_t stream);
+
+/* y = act(x[:, :k]) * x[:, k:] (gate_act 1 silu, 2 gelu_tanh) of x [rows, 2 k] bf16 /
+ * fp16 / fp32 (in_type 0 / 1 / 2), in fp32, into 8 bits: q and scales as in
+ * strix_rms_norm_quant. The step between the two GEMMs of a W8A8 MLP; in the
+ * reference vLLM's silu_and_mul and the GEMM's own quantiser
+ * (csrc/gemm/w8a8_wmma_gemm.hip:508-529). */
+int strix_act_mul_quant(const void* x, void* q, float* scales, int64_t rows, int64_t k,
+                        int64_t x_stride, int64_t q_stride, int64_t s_stride, int gate_act,
+                        int in_type, int fp8, strix_stream_t stream);
+
 /* ------------------------------------------------------------------------
  * Prefill attention: causal paged flash attention over ragged sequences.
  * Replaces strix::attn_prefill_bf16 (csrc/attn/attn_prefill_bf16.hip:508-662;

@@ -19,7 +19,7 @@ from .registry import Range, explain, geometries, kernels, ops, select, selectio
 
 _lib.load()
 from . import torch_ops  # noqa: E402  (registers torch.ops.strix.*)
-from . import moe  # noqa: E402
+from . import dense, moe  # noqa: E402
 
 StrixError = _lib.StrixError
 
@@ -133,6 +133,7 @@ __all__ = [
     "Range",
     "StrixError",
     "attn_decode",
+    "dense",
     "explain",
     "geometries",
     "is_supported_device",

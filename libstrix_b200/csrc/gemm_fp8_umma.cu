@@ -1,0 +1,373 @@
+// Dense FP8 W8A8 product with a scale per block of 128, on tcgen05 kind::f8f6f4:
+//
+//   out[m, n] = sum_b sa[m, b] * sw[n / 128, b] * (sum_{k in block b} a[m, k] w[n, k]) (+ bias[n])
+//
+// a e4m3 [M, K] with one fp32 scale per (row, 128 columns), w e4m3 [N, K] with one
+// per 128 x 128 block. The scales are arbitrary fp32 numbers and cannot ride the MMA
+// (its block scales are powers of two), so each K block of 128 is one fresh
+// accumulation in tensor memory, and the epilogue warps fold it into fp32 registers:
+// acc += partial * (sa * sw). The reference has this product with 16-bit activations
+// only (csrc/gemm/fp8_wmma_gemm.hip; the schema at csrc/torch_ops.cpp:256).
+//
+// K that is no multiple of 128: the TMA fills the last block with zero bytes, which
+// are zeros of e4m3. Rows past M or N arrive as zeros and are not stored.
+#include "cluster.cuh"
+#include "tma.cuh"
+
+namespace strix {
+
+int32_t* umma_status_ptr();  // moe_gemm_umma.cu: device address of the shared status word
+
+namespace {
+
+using namespace umma;
+
+constexpr int kBlk = 128;          // K block, bytes and columns alike
+
+enum OutKind : int { kOutBf16 = 0, kOutF16 = 1, kOutF32 = 2 };
+
+struct Fp8GemmArgs {
+  void* out;                       // [M, N], row stride out_st
+  const float *sa, *sw;
+  const void* bias;                // NULL or [N], in the output's type
+  int32_t* status;
+  int64_t out_st, sa_sm, sa_sk, sw_sn, sw_sk;
+  int M, N, nkb;
+  int n_tiles, splits;             // stream kernel: 128-row weight tiles, CTAs per tile along K
+  int out_kind;
+};
+
+__device__ __forceinline__ float load_bias(const void* bias, int kind, int n) {
+  if (bias == nullptr) return 0.f;
+  if (kind == kOutBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[n]);
+  if (kind == kOutF16) return __half2float(static_cast<const __half*>(bias)[n]);
+  return static_cast<const float*>(bias)[n];
+}
+
+__device__ __forceinline__ void store_one(void* out, int kind, int64_t at, float v) {
+  if (kind == kOutBf16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else if (kind == kOutF16) static_cast<__half*>(out)[at] = __float2half_rn(v);
+  else static_cast<float*>(out)[at] = v;
+}
+
+// ================================================================ weight stream
+// Few tokens: the weights are the MMA's A operand (128 rows fill M whatever the
+// batch), NB tokens its N, and the kernel is a stream of the weights. A cluster of
+// `splits` CTAs shares one tile of 128 weight rows along K and adds its partial sums
+// through distributed shared memory in rank order, so a layer with few tiles still
+// fills the GPU, the result does not depend on timing and no scratch is needed.
+// Warp 0 loads (TMA), warp 1 issues, warp 2 stages the tokens' scales, warps 4-7
+// fold. Two CTAs share an SM, so one's start and join hide behind the other's stream.
+constexpr int kStreamThreads = 256;
+
+template <int NB>
+struct StreamLayout {
+  static constexpr int kWBytes = 128 * kBlk, kTBytes = NB * kBlk;
+  static constexpr int kStageBytes = kWBytes + kTBytes;
+  static constexpr int kStages = (100 * 1024) / kStageBytes;
+  static constexpr int kAcc = 4;                                   // accumulators in tensor memory
+  static constexpr int kTmemCols = kAcc * NB < 32 ? 32 : kAcc * NB;
+  static constexpr int kSmem = 1024 + kStages * (kStageBytes + NB * 4);
+  static_assert(kStages * kStageBytes >= NB * 128 * 4, "the join reuses the ring");
+};
+
+template <int NB>
+__global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
+    const Fp8GemmArgs p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a) {
+  pdl_enter();
+  using L = StreamLayout<NB>;
+  constexpr int S = L::kStages, NA = L::kAcc;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  float* s_scale = reinterpret_cast<float*>(ring + S * L::kStageBytes);    // [S][NB]
+  __shared__ __align__(8) uint64_t full_bar[S], done_bar[S], sfull_bar[S], sempty_bar[S], tempty_bar[NA], drain_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int s_abort;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = int(blockIdx.x) % p.splits, tile = int(blockIdx.x) / p.splits;
+  const int n0 = (tile % p.n_tiles) * 128, m0 = (tile / p.n_tiles) * NB;
+  // K blocks [k0, k0 + nk) of this CTA
+  const int base = p.nkb / p.splits, rem = p.nkb % p.splits;
+  const int nk = base + (rank < rem ? 1 : 0), k0 = rank * base + min(rank, rem);
+  int armed = 0;
+
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full_bar[i], 1), mbar_init(&done_bar[i], 1);
+      mbar_init(&sfull_bar[i], 32), mbar_init(&sempty_bar[i], 4);
+    }
+    for (int i = 0; i < NA; ++i) mbar_init(&tempty_bar[i], 4);
+    mbar_init(&drain_bar, 1);
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&tmem_slot, L::kTmemCols);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot, ring_s = smem_u32(ring);
+
+  constexpr int NC = NB;
+  float acc[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma::prefetch_map(&map_w);
+      tma::prefetch_map(&map_a);
+      bool dead = false;
+      int t = 0;
+      for (; t < nk; ++t) {
+        const int s = t % S;
+        if (!mbar_wait(&done_bar[s], ((t / S) & 1) ^ 1) || s_abort) {
+          dead = true;
+          break;
+        }
+        const uint32_t st = ring_s + s * L::kStageBytes;
+        tma::mbar_expect_tx(&full_bar[s], L::kStageBytes);
+        tma::load_2d(st, &map_w, (k0 + t) * kBlk, n0, &full_bar[s]);
+        tma::load_2d(st + L::kWBytes, &map_a, (k0 + t) * kBlk, m0, &full_bar[s]);
+      }
+      armed = t;
+      if (dead) atomicExch(p.status, 1), s_abort = 1;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc(D_F32, 0, 0, 128, NB);
+      const uint32_t w_lo0 = smem_desc_lo(ring_s);
+      bool dead = false;
+      for (int t = 0; t < nk; ++t) {
+        const int s = t % S, b = t % NA;
+        const bool ok_full = mbar_wait(&full_bar[s], (t / S) & 1);
+        const bool ok_acc = mbar_wait(&tempty_bar[b], ((t / NA) & 1) ^ 1);
+        if (!ok_full || !ok_acc || s_abort) {
+          dead = true;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t w_lo = w_lo0 + s * (L::kStageBytes >> 4), t_lo = w_lo + (L::kWBytes >> 4);
+        const uint32_t d = tmem + b * NB;
+        mma_ss_lo<KIND_F8F6F4, false>(d, w_lo, t_lo, idesc);
+        mma_ss_lo<KIND_F8F6F4, true>(d, w_lo + 2, t_lo + 2, idesc);
+        mma_ss_lo<KIND_F8F6F4, true>(d, w_lo + 4, t_lo + 4, idesc);
+        mma_ss_lo<KIND_F8F6F4, true>(d, w_lo + 6, t_lo + 6, idesc);
+        mma_commit(&done_bar[s]);   // frees the stage and publishes the sums
+      }
+      if (dead) atomicExch(p.status, 1), s_abort = 1;
+    }
+  } else if (warp == 2) {
+    // the tokens' scales of one K block per ring position, copied ahead
+    bool dead = false;
+    for (int t = 0; t < nk; ++t) {
+      const int s = t % S;
+      const bool ok = mbar_wait(&sempty_bar[s], ((t / S) & 1) ^ 1);
+      if (__any_sync(0xffffffffu, !ok || s_abort != 0)) {
+        dead = true;
+        break;
+      }
+      for (int j = lane; j < NB; j += 32) {
+        const bool live = m0 + j < p.M;
+        cp_async_4_zfill(smem_u32(s_scale + s * NB + j),
+                         p.sa + (live ? int64_t(m0 + j) * p.sa_sm + int64_t(k0 + t) * p.sa_sk : 0), live);
+      }
+      mbar_arrive_cp_async(&sfull_bar[s]);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();   // nothing of this warp is in flight when the CTA ends
+    if (dead && lane == 0) atomicExch(p.status, 1), s_abort = 1;
+  } else if (warp >= 4) {
+    const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
+    const float* sw = p.sw + int64_t(n0 / kBlk) * p.sw_sn + int64_t(k0) * p.sw_sk;
+    float w_next = nk > 0 ? __ldg(sw) : 0.f;
+    bool dead = false;
+    for (int t = 0; t < nk; ++t) {
+      const int s = t % S, b = t % NA;
+      const float ws = w_next;
+      if (t + 1 < nk) w_next = __ldg(sw + int64_t(t + 1) * p.sw_sk);
+      const bool ok_s = mbar_wait(&sfull_bar[s], (t / S) & 1);
+      const bool ok_d = mbar_wait(&done_bar[s], (t / S) & 1);
+      if (__any_sync(0xffffffffu, !ok_s || !ok_d || s_abort != 0)) {
+        dead = true;
+        break;
+      }
+      tc_fence_after_sync();
+      const float4* sc = reinterpret_cast<const float4*>(s_scale + s * NB);
+#pragma unroll
+      for (int c = 0; c < NC; c += 16) {
+        uint32_t r[16];
+        tmem_ld_32x16(tmem + lane_base + b * NB + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 q = sc[(c + j) >> 2];
+          acc[c + j] += __uint_as_float(r[j]) * (q.x * ws);
+          acc[c + j + 1] += __uint_as_float(r[j + 1]) * (q.y * ws);
+          acc[c + j + 2] += __uint_as_float(r[j + 2]) * (q.z * ws);
+          acc[c + j + 3] += __uint_as_float(r[j + 3]) * (q.w * ws);
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty_bar[b]), mbar_arrive(&sempty_bar[s]);
+    }
+    if (dead) atomicExch(p.status, 1), s_abort = 1;
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (s_abort) {   // wait for the copies and MMAs still in flight before TMEM and the ring go
+    if (tid == 0) drain_armed_loads(full_bar, S, armed);
+    if (warp == 1 && lane == 0) drain_issued_mmas(&drain_bar);
+    tc_fence_before_sync();
+    __syncthreads();
+  }
+  if (warp == 1) tmem_dealloc(tmem, L::kTmemCols);
+
+  // thread r of warps 4-7 holds the sums of weight row n0 + r for the NB tokens
+  const int row = (warp & 3) * 32 + lane, n = n0 + row;
+  const bool n_ok = n < p.N;
+  if (p.splits == 1) {
+    if (warp >= 4 && n_ok) {
+      const float bias = load_bias(p.bias, p.out_kind, n);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        if (m0 + j < p.M) store_one(p.out, p.out_kind, int64_t(m0 + j) * p.out_st + n, acc[j] + bias);
+    }
+    return;
+  }
+  // the join: every CTA lays its partial tile [token][row] into its ring (whose copies and
+  // MMAs have ended), then sums the tokens rank, rank + splits, ... over the cluster
+  float* part = reinterpret_cast<float*>(ring);
+  if (warp >= 4) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) part[j * 128 + row] = acc[j];
+  }
+  cluster::sync();
+  {
+    const int r = tid & 127, col = n0 + r;
+    const float bias = col < p.N ? load_bias(p.bias, p.out_kind, col) : 0.f;
+    const uint32_t own = smem_u32(part);
+    for (int j = rank * 2 + (tid >> 7); j < NB; j += 2 * p.splits) {
+      if (m0 + j >= p.M) break;
+      float v = 0.f;
+      for (int c = 0; c < p.splits; ++c) v += cluster::ld_shared_f32(cluster::map_shared(own + (j * 128 + r) * 4, c));
+      if (col < p.N) store_one(p.out, p.out_kind, int64_t(m0 + j) * p.out_st + col, v + bias);
+    }
+  }
+  cluster::sync();   // nobody leaves while a peer still reads its shared memory
+}
+
+template <int NB>
+int launch_stream(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
+                  int dev, cudaStream_t st) {
+  using L = StreamLayout<NB>;
+  auto kernel = gemm_fp8_stream_kernel<NB>;
+  static bool done[64] = {};
+  if (!done[dev]) {
+    STRIX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
+    done[dev] = true;
+  }
+  p.n_tiles = (p.N + 127) / 128;
+  const int64_t tiles = int64_t(p.n_tiles) * ((p.M + NB - 1) / NB);
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 2 * sms && p.nkb >= splits * 2) splits *= 2;
+  p.splits = splits;
+  STRIX_CHECK(tiles * splits < (int64_t(1) << 31), "matrix too large");
+  CUtensorMap map_w, map_a;
+  STRIX_CHECK(tma::make_map_u8(&map_w, w, uint64_t(p.N), uint64_t(k), uint64_t(w_st), 128) &&
+                  tma::make_map_u8(&map_a, a, uint64_t(p.M), uint64_t(k), uint64_t(a_st), NB),
+              "tensor map encoding failed");
+  STRIX_CUDA(cluster::launch(kernel, unsigned(tiles * splits), unsigned(splits), kStreamThreads, L::kSmem, st, p, map_w, map_a));
+  return launch_status("w8a8_fp8_gemm");
+}
+
+// The checks that both entry points share; fills what the kernels read of the operands.
+int fp8_operands(Fp8GemmArgs& p, const void* a_q, const float* a_scale, const void* w, const float* w_scale,
+                 int64_t m, int64_t n, int64_t k, int64_t& a_stride, int64_t& w_stride, int& dev, int& sms) {
+  STRIX_CHECK(m >= 0 && n > 0 && k > 0, "bad shapes");
+  STRIX_CHECK(k % 16 == 0, "K must be a multiple of 16");
+  STRIX_CHECK(n < (int64_t(1) << 31) - 256 && m < (int64_t(1) << 31) - 256 && k < (int64_t(1) << 31) - 256,
+              "matrix too large");
+  if (m == 0) return STRIX_OK;
+  STRIX_CHECK(a_q != nullptr && a_scale != nullptr && w != nullptr && w_scale != nullptr,
+              "pointers must not be NULL");
+  // the stride of a single row is not read, but a tensor map wants a valid one
+  if (m == 1) a_stride = k;
+  if (n == 1) w_stride = k;
+  STRIX_CHECK(a_stride % 16 == 0 && w_stride % 16 == 0 && reinterpret_cast<uintptr_t>(a_q) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(w) % 16 == 0,
+              "16-byte aligned rows required");
+  STRIX_CHECK(a_stride >= k && w_stride >= k && a_stride < (int64_t(1) << 40) && w_stride < (int64_t(1) << 40),
+              "rows must not overlap");
+  p.sa = a_scale, p.sw = w_scale;
+  p.status = umma_status_ptr();
+  STRIX_CHECK(p.status != nullptr, "status word unavailable");
+  p.M = int(m), p.N = int(n), p.nkb = int((k + kBlk - 1) / kBlk);
+  static int sm_count[64] = {};
+  STRIX_CUDA(cudaGetDevice(&dev));
+  STRIX_CHECK(dev >= 0 && dev < 64, "device index %d out of range", dev);
+  if (!sm_count[dev]) STRIX_CUDA(cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev));
+  sms = sm_count[dev];
+  return STRIX_OK;
+}
+
+int run_gemm(const Fp8GemmArgs& p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
+             int dev, cudaStream_t st) {
+  if (p.M <= 16) return launch_stream<16>(p, a, a_st, w, w_st, k, sms, dev, st);
+  if (p.M <= 32) return launch_stream<32>(p, a, a_st, w, w_st, k, sms, dev, st);
+  return launch_stream<64>(p, a, a_st, w, w_st, k, sms, dev, st);
+}
+
+}  // namespace
+}  // namespace strix
+
+using namespace strix;
+
+extern "C" int strix_w8a8_fp8_gemm(void* out, const void* a_q, const float* a_scale, const void* w,
+                                   const float* w_scale, const void* bias, int64_t m, int64_t n, int64_t k,
+                                   int64_t a_stride, int64_t w_stride, int64_t out_stride,
+                                   int64_t sa_stride_m, int64_t sa_stride_k, int64_t sw_stride_n,
+                                   int64_t sw_stride_k, int out_kind, strix_stream_t stream) {
+  STRIX_CHECK(out_kind >= 0 && out_kind <= 2, "output must be bf16, fp16 or fp32");
+  Fp8GemmArgs p{};
+  int dev = 0, sms = 0;
+  const int rc = fp8_operands(p, a_q, a_scale, w, w_scale, m, n, k, a_stride, w_stride, dev, sms);
+  if (rc != STRIX_OK || m == 0) return rc;
+  STRIX_CHECK(out != nullptr && (m == 1 || out_stride >= n), "output rows must not overlap");
+  p.out = out, p.bias = bias, p.out_kind = out_kind;
+  p.out_st = out_stride, p.sa_sm = sa_stride_m, p.sa_sk = sa_stride_k;
+  p.sw_sn = sw_stride_n, p.sw_sk = sw_stride_k;
+  return run_gemm(p, a_q, a_stride, w, w_stride, k, sms, dev, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t strix_w8a8_fp8_gated_workspace(int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n <= 0 || k <= 0 || m >= (int64_t(1) << 31) || n >= (int64_t(1) << 30)) return -1;
+  return m * 2 * n * 4;
+}
+
+extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, const float* a_scale,
+                                    const void* w, const float* w_scale, void* workspace,
+                                    int64_t workspace_bytes, int64_t m, int64_t n, int64_t k,
+                                    int64_t a_stride, int64_t w_stride, int64_t q_stride, int64_t s_stride,
+                                    int64_t sa_stride_m, int64_t sa_stride_k, int64_t sw_stride_n,
+                                    int64_t sw_stride_k, int gate_act, strix_stream_t stream) {
+  STRIX_CHECK(gate_act == 1 || gate_act == 2, "activation must be silu or gelu_tanh");
+  STRIX_CHECK(n > 0 && n < (int64_t(1) << 30) && n % 16 == 0, "N must be a multiple of 16");
+  Fp8GemmArgs p{};
+  int dev = 0, sms = 0;
+  int rc = fp8_operands(p, a_q, a_scale, w, w_scale, m, 2 * n, k, a_stride, w_stride, dev, sms);
+  if (rc != STRIX_OK || m == 0) return rc;
+  STRIX_CHECK(q != nullptr && scales != nullptr, "pointers must not be NULL");
+  STRIX_CHECK(reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride % 16 == 0, "16-byte aligned rows required");
+  STRIX_CHECK(m == 1 || (q_stride >= n && s_stride >= (n + 127) / 128), "output rows must not overlap");
+  const int64_t need = strix_w8a8_fp8_gated_workspace(m, n, k);
+  STRIX_CHECK(workspace_bytes >= need && (need == 0 || (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0)),
+              "workspace must hold %lld bytes on a 16-byte boundary", (long long)need);
+  p.out = workspace, p.out_kind = kOutF32, p.out_st = 2 * n;
+  p.sa_sm = sa_stride_m, p.sa_sk = sa_stride_k, p.sw_sn = sw_stride_n, p.sw_sk = sw_stride_k;
+  rc = run_gemm(p, a_q, a_stride, w, w_stride, k, sms, dev, static_cast<cudaStream_t>(stream));
+  if (rc != STRIX_OK) return rc;
+  return strix_act_mul_quant(workspace, q, scales, m, n, 2 * n, q_stride, s_stride, gate_act, 2, 1, stream);
+}

@@ -1,0 +1,77 @@
+"""The 8-bit dense layer built from the strix ops: norm (with the residual's addition)
+into 8 bits, the W8A8 products, the gated activation into 8 bits, and the MLP that runs
+them one after the other.
+
+Two forms, by what the weights are: FP8 (e4m3, one fp32 scale per 128 x 128 block;
+activations e4m3 with one per (row, 128 columns)) and int8 (one scale per output
+channel; activations int8 with one per row). In the reference the linear layers take
+16-bit activations and quantise inside (csrc/gemm/w8a8_wmma_gemm.hip:508-529,
+python/strix_vllm/fp8.py:121-262), with vLLM's 16-bit norm and silu_and_mul between.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import torch_ops  # noqa: F401  (registers torch.ops.strix.*)
+
+FP8 = torch.float8_e4m3fn
+
+
+def _is_fp8(q_dtype: torch.dtype) -> bool:
+    if q_dtype not in (FP8, torch.int8):
+        raise RuntimeError(f"q_dtype must be float8_e4m3fn or int8, got {q_dtype}")
+    return q_dtype == FP8
+
+
+def rms_norm_quant(x, weight, eps: float = 1e-6, residual=None, residual_out=None, q_dtype=FP8):
+    """(q, scales) of rms_norm(x + residual) * weight.
+
+    x, residual: [M, K] bf16 / fp16; weight [K] of the same dtype or fp32. residual_out
+    receives x + residual rounded to x's dtype: a tensor of its own, or x or residual
+    itself for an update in place. The norm is taken of the fp32 sum, before that
+    rounding. q_dtype float8_e4m3fn: scales fp32 [M, ceil(K / 128)], K a multiple of 16;
+    int8: scales fp32 [M], K a multiple of 8."""
+    op = torch.ops.strix.rms_norm_quant_fp8 if _is_fp8(q_dtype) else torch.ops.strix.rms_norm_quant_token_i8
+    return op(x, weight, eps, residual, residual_out)
+
+
+def act_mul_quant(x, activation: str = "silu", q_dtype=FP8):
+    """(q, scales) of act(x[:, :K]) * x[:, K:] for x [M, 2 K] (bf16, fp16 or fp32),
+    activation silu or gelu_tanh; q and scales as rms_norm_quant returns them."""
+    op = torch.ops.strix.act_mul_quant_fp8 if _is_fp8(q_dtype) else torch.ops.strix.act_mul_quant_token_i8
+    return op(x, activation)
+
+
+def fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
+    """[M, N] of a_q e4m3 [M, K] (a_scale fp32 [M, ceil(K / 128)]) and w e4m3 [N, K]
+    (w_scale fp32 [ceil(N / 128), ceil(K / 128)]), K a multiple of 16."""
+    return torch.ops.strix.w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias, out_dtype)
+
+
+def fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation: str = "silu"):
+    """(q e4m3 [M, N], scales) of act(gate) * up, where w e4m3 [2 N, K] holds the gate
+    rows and then the up rows: fp8_gemm and act_mul_quant without the 16-bit rows
+    between them."""
+    return torch.ops.strix.w8a8_fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation)
+
+
+def fused_mlp_fp8_w8a8(x, norm_weight, w13, w13_scale, w2, w2_scale, eps: float = 1e-6, residual=None,
+                       residual_out=None, activation: str = "silu"):
+    """One MLP block in FP8 W8A8: norm (x + residual) -> gate-up product with the gate
+    -> down product. x [T, H] bf16 / fp16; w13 e4m3 [2 I, H], w2 e4m3 [H, I] with fp32
+    128 x 128 block scales. Returns [T, H] of x's dtype (the residual stream's increment;
+    the stream itself is residual_out)."""
+    q, s = rms_norm_quant(x, norm_weight, eps, residual, residual_out)
+    q, s = fp8_gemm_act_mul_quant(q, s, w13, w13_scale, activation)
+    return fp8_gemm(q, s, w2, w2_scale, None, x.dtype)
+
+
+def fused_mlp_int8_w8a8(x, norm_weight, w13, w13_scale, w2, w2_scale, eps: float = 1e-6, residual=None,
+                        residual_out=None, activation: str = "silu"):
+    """The same block over int8 weights [2 I, H] and [H, I] with one fp32 scale per output
+    channel (H and I multiples of 128). Returns bf16 [T, H]."""
+    q, s = rms_norm_quant(x, norm_weight, eps, residual, residual_out, torch.int8)
+    h = torch.ops.strix.w8a8_int8_gemm(q, s, w13, w13_scale)
+    q, s = act_mul_quant(h, activation, torch.int8)
+    return torch.ops.strix.w8a8_int8_gemm(q, s, w2, w2_scale)

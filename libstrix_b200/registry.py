@@ -317,6 +317,36 @@ KERNELS: list[Kernel] = [
            "dynamic symmetric per-token int8 activations (scale = absmax / 127), the input "
            "form of w8a8_int8_gemm",
            {"dtype": ("bf16", "fp16"), "activation_dtype": "int8", "group_size": 0}),
+    # ---------------------------------------------------- 8-bit dense layer
+    Kernel("w8a8_fp8_gemm", "fp8_w8a8",
+           "dense FP8 W8A8 product on tcgen05 kind::f8f6f4: e4m3 activations with one fp32 scale "
+           "per (row, 128 columns), e4m3 weights with one per 128 x 128 block, folded in fp32 per K "
+           "block. K % 16 == 0, any M and N, bias per channel",
+           {"weight_bits": 8, "weight_dtype": "fp8_e4m3", "act_dtype": "fp8_e4m3", "group_size": 128,
+            "dtype": ("bf16", "fp16", "fp32")},
+           {"tile": "128 weights x 16/32/64 tokens, up to 8 CTAs per tile along K joined through "
+                    "distributed shared memory",
+            "bound": "hbm"}),
+    Kernel("w8a8_fp8_gemm_act_mul_quant", "fp8_w8a8_gated",
+           "the gate-up form of w8a8_fp8_gemm: act(gate) * up of the fp32 sums, out as e4m3 with "
+           "one scale per (row, 128 columns)",
+           {"weight_bits": 8, "weight_dtype": "fp8_e4m3", "act_dtype": "fp8_e4m3", "group_size": 128,
+            "activation": ("silu", "gelu_tanh")},
+           {"bound": "hbm"}),
+    *[Kernel(f"rms_norm_quant_{form}", "rms_norm_quant",
+             "root-mean-square norm with the residual's addition, out in 8 bits with scales; a row "
+             "is read once and stays in registers",
+             {"dtype": ("bf16", "fp16"), "activation_dtype": q, "group_size": group,
+              "residual": (True, False)},
+             {"unit": "one CTA per row", "bound": "hbm"})
+      for form, q, group in (("fp8", "fp8_e4m3", 128), ("token_i8", "int8", 0))],
+    *[Kernel(f"act_mul_quant_{form}", "act_mul_quant",
+             "act(gate) * up of gate-up rows, out in 8 bits with scales",
+             {"dtype": ("bf16", "fp16", "fp32"), "activation_dtype": q, "group_size": group,
+              "activation": ("silu", "gelu_tanh")},
+             {"unit": unit, "bound": "hbm"})
+      for form, q, group, unit in (("fp8", "fp8_e4m3", 128, "16 lanes per (row, 128 columns)"),
+                                   ("token_i8", "int8", 0, "one CTA per row"))],
     # ------------------------------------------------------------ attention
     Kernel("kv_write_i8", "kv_write",
            "new K/V rows quantised per (token, KV head) into the int8 paged cache with their "

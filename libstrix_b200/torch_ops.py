@@ -1124,6 +1124,181 @@ def act_quant_token_i8(x):
     return q, s
 
 
+# ------------------------------------------- 8-bit dense layer (not in the reference)
+# The steps around the W8A8 products - vLLM runs them there in 16 bits, and the
+# reference's GEMMs quantise their own activations
+# (csrc/gemm/w8a8_wmma_gemm.hip:508-529) - and the FP8 product with 8-bit activations.
+
+_OUT_KINDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _groups(k: int) -> int:
+    return (k + 127) // 128
+
+
+def _same_device(*tensors) -> None:
+    dev = tensors[0].device
+    _check(all(t is None or t.device == dev for t in tensors), "tensors must be on one device")
+
+
+def _norm_fake(x, weight, eps, residual=None, residual_out=None):
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty((x.size(0), _groups(x.size(1))), dtype=torch.float32))
+
+
+def _norm_i8_fake(x, weight, eps, residual=None, residual_out=None):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty((x.size(0),), dtype=torch.float32)
+
+
+def _rms_norm_quant(x, weight, eps, residual, residual_out, fp8):
+    _check(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float16) and x.stride(1) == 1,
+           "x must be bf16 or fp16 [rows, K] with contiguous rows")
+    m, k = x.shape
+    _check(k > 0 and k % (16 if fp8 else 8) == 0, f"K must be a multiple of {16 if fp8 else 8}")
+    _check(weight.dim() == 1 and weight.size(0) == k and weight.dtype in (x.dtype, torch.float32)
+           and weight.stride(0) == 1, "weight must be contiguous [K], of x's dtype or fp32")
+    _check(eps >= 0, "eps must not be negative")
+    _check(residual_out is None or residual is not None, "residual_out needs a residual")
+    for name, t in (("residual", residual), ("residual_out", residual_out)):
+        _check(t is None or (t.dtype == x.dtype and t.shape == x.shape and t.stride(1) == 1),
+               f"{name} must match x")
+    _same_device(x, weight, residual, residual_out)
+    q = torch.empty((m, k), dtype=torch.float8_e4m3fn if fp8 else torch.int8, device=x.device)
+    s = torch.empty((m, _groups(k)) if fp8 else (m,), dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.call("strix_rms_norm_quant", x.data_ptr(), _ptr(residual), _ptr(residual_out),
+                  weight.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0),
+                  0 if residual is None else residual.stride(0),
+                  0 if residual_out is None else residual_out.stride(0), k, s.stride(0), eps,
+                  int(x.dtype == torch.float16), int(weight.dtype == torch.float32), int(fp8), _stream())
+    return q, s
+
+
+@_define("rms_norm_quant_fp8(Tensor x, Tensor weight, float eps, Tensor? residual=None, "
+         "Tensor(a!)? residual_out=None) -> (Tensor, Tensor)", fake=_norm_fake)
+def rms_norm_quant_fp8(x, weight, eps, residual=None, residual_out=None):
+    """(q e4m3 [M, K], scales fp32 [M, ceil(K / 128)]) of rms_norm(x + residual) * weight,
+    the activation form of w8a8_fp8_gemm; residual_out receives the sum in x's dtype."""
+    return _rms_norm_quant(x, weight, eps, residual, residual_out, True)
+
+
+@_define("rms_norm_quant_token_i8(Tensor x, Tensor weight, float eps, Tensor? residual=None, "
+         "Tensor(a!)? residual_out=None) -> (Tensor, Tensor)", fake=_norm_i8_fake)
+def rms_norm_quant_token_i8(x, weight, eps, residual=None, residual_out=None):
+    """(q int8 [M, K], scale fp32 [M]) of rms_norm(x + residual) * weight, the activation
+    form of w8a8_int8_gemm; residual_out receives the sum in x's dtype."""
+    return _rms_norm_quant(x, weight, eps, residual, residual_out, False)
+
+
+def _act_mul_fake(x, activation="silu"):
+    k = x.size(1) // 2
+    return (x.new_empty((x.size(0), k), dtype=torch.float8_e4m3fn),
+            x.new_empty((x.size(0), _groups(k)), dtype=torch.float32))
+
+
+def _act_mul_i8_fake(x, activation="silu"):
+    return (x.new_empty((x.size(0), x.size(1) // 2), dtype=torch.int8),
+            x.new_empty((x.size(0),), dtype=torch.float32))
+
+
+def _act_mul_quant(x, activation, fp8):
+    _check(x.dim() == 2 and x.dtype in _OUT_KINDS and x.stride(1) == 1,
+           "x must be bf16, fp16 or fp32 [rows, 2 K] with contiguous rows")
+    _check(activation in _ACTS, f"activation must be silu or gelu_tanh, got {activation}")
+    m, k = x.size(0), x.size(1) // 2
+    _check(x.size(1) % 2 == 0 and k > 0 and k % (16 if fp8 else 8) == 0,
+           f"K must be a multiple of {16 if fp8 else 8}")
+    q = torch.empty((m, k), dtype=torch.float8_e4m3fn if fp8 else torch.int8, device=x.device)
+    s = torch.empty((m, _groups(k)) if fp8 else (m,), dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.call("strix_act_mul_quant", x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0), k,
+                  s.stride(0), _ACTS[activation], _OUT_KINDS[x.dtype], int(fp8), _stream())
+    return q, s
+
+
+@_define("act_mul_quant_fp8(Tensor x, str activation='silu') -> (Tensor, Tensor)", fake=_act_mul_fake)
+def act_mul_quant_fp8(x, activation="silu"):
+    """(q e4m3 [M, K], scales fp32 [M, ceil(K / 128)]) of act(x[:, :K]) * x[:, K:]."""
+    return _act_mul_quant(x, activation, True)
+
+
+@_define("act_mul_quant_token_i8(Tensor x, str activation='silu') -> (Tensor, Tensor)",
+         fake=_act_mul_i8_fake)
+def act_mul_quant_token_i8(x, activation="silu"):
+    """(q int8 [M, K], scale fp32 [M]) of act(x[:, :K]) * x[:, K:]."""
+    return _act_mul_quant(x, activation, False)
+
+
+def _fp8_operands(a_q, a_scale, w, w_scale):
+    f8 = torch.float8_e4m3fn
+    _check(a_q.dim() == 2 and w.dim() == 2 and a_q.dtype == f8 and w.dtype == f8
+           and a_q.size(1) == w.size(1) and a_q.stride(1) == 1 and w.stride(1) == 1,
+           "a_q, w must be float8_e4m3fn [M, K], [N, K] with contiguous rows")
+    m, k = a_q.shape
+    n = w.size(0)
+    _check(n > 0 and k > 0 and k % 16 == 0, "K must be a multiple of 16")
+    _check(a_scale.dtype == torch.float32 and tuple(a_scale.shape) == (m, _groups(k)),
+           "a_scale must be fp32 [M, ceil(K/128)]")
+    _check(w_scale.dtype == torch.float32 and tuple(w_scale.shape) == (_groups(n), _groups(k)),
+           "block scales must be fp32 [ceil(N/128), ceil(K/128)]")
+    _same_device(a_q, a_scale, w, w_scale)
+    return m, n, k
+
+
+def _w8a8_fp8_fake(a_q, a_scale, w, w_scale, bias=None, out_dtype=None):
+    return a_q.new_empty((a_q.size(0), w.size(0)), dtype=out_dtype or torch.bfloat16)
+
+
+@_define("w8a8_fp8_gemm(Tensor a_q, Tensor a_scale, Tensor w, Tensor w_scale, Tensor? bias=None, "
+         "ScalarType? out_dtype=None) -> Tensor", fake=_w8a8_fp8_fake)
+def w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=None):
+    """out [M, N] (bf16, or out_dtype fp16 / fp32) of e4m3 activations with one fp32 scale
+    per (row, 128 columns) and e4m3 weights with one per 128 x 128 block; bias [N] of the
+    output's dtype."""
+    m, n, k = _fp8_operands(a_q, a_scale, w, w_scale)
+    out_dtype = out_dtype or torch.bfloat16
+    _check(out_dtype in _OUT_KINDS, "out_dtype must be bf16, fp16 or fp32")
+    if bias is not None:
+        _check(bias.dtype == out_dtype and tuple(bias.shape) == (n,) and bias.stride(0) == 1,
+               "bias must be contiguous [N] of the output's dtype")
+        _same_device(a_q, bias)
+    out = torch.empty((m, n), dtype=out_dtype, device=a_q.device)
+    with torch.cuda.device(a_q.device):
+        _lib.call("strix_w8a8_fp8_gemm", out.data_ptr(), a_q.data_ptr(), a_scale.data_ptr(), w.data_ptr(),
+                  w_scale.data_ptr(), _ptr(bias), m, n, k, a_q.stride(0), w.stride(0), n,
+                  *a_scale.stride(), *w_scale.stride(), _OUT_KINDS[out_dtype], _stream())
+        _lib.after_tcgen05("w8a8_fp8_gemm")
+    return out
+
+
+def _gated_fake(a_q, a_scale, w, w_scale, activation="silu"):
+    n = w.size(0) // 2
+    return (a_q.new_empty((a_q.size(0), n)),
+            a_q.new_empty((a_q.size(0), _groups(n)), dtype=torch.float32))
+
+
+@_define("w8a8_fp8_gemm_act_mul_quant(Tensor a_q, Tensor a_scale, Tensor w, Tensor w_scale, "
+         "str activation='silu') -> (Tensor, Tensor)", fake=_gated_fake)
+def w8a8_fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation="silu"):
+    """The gate-up product that ends in the down product's input: w e4m3 [2 N, K] holds the
+    gate rows, then the up rows; (q e4m3 [M, N], scales fp32 [M, ceil(N / 128)]) of
+    act(gate) * up, taken from the fp32 sums without a 16-bit step in between."""
+    m, n2, k = _fp8_operands(a_q, a_scale, w, w_scale)
+    _check(activation in _ACTS, f"activation must be silu or gelu_tanh, got {activation}")
+    n = n2 // 2
+    _check(n2 % 32 == 0, "w must hold gate and up rows, a multiple of 16 each")
+    q = torch.empty((m, n), dtype=torch.float8_e4m3fn, device=a_q.device)
+    s = torch.empty((m, _groups(n)), dtype=torch.float32, device=a_q.device)
+    nbytes = _lib.load().strix_w8a8_fp8_gated_workspace(m, n, k)
+    with torch.cuda.device(a_q.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=a_q.device) if nbytes > 0 else None
+        _lib.call("strix_w8a8_fp8_gated", q.data_ptr(), s.data_ptr(), a_q.data_ptr(), a_scale.data_ptr(),
+                  w.data_ptr(), w_scale.data_ptr(), _ptr(ws), nbytes, m, n, k, a_q.stride(0), w.stride(0), n,
+                  s.stride(0), *a_scale.stride(), *w_scale.stride(), _ACTS[activation], _stream())
+        _lib.after_tcgen05("w8a8_fp8_gemm_act_mul_quant")
+    return q, s
+
+
 # ----------------------------------------------------------- tcgen05 layout probe
 
 def _umma_tile_fake(a, b):
