@@ -34,7 +34,7 @@ struct Fp8GemmArgs {
   int64_t out_st, sa_sm, sa_sk, sw_sn, sw_sk;
   int M, N, nkb;
   int n_tiles, splits;             // stream kernel: 128-row weight tiles, CTAs per tile along K
-  int out_kind;
+  int out_kind, tma_out;           // tma_out: the wide kernel's rows may leave by TMA (16-byte boundaries)
 };
 
 __device__ __forceinline__ float load_bias(const void* bias, int kind, int n) {
@@ -283,6 +283,302 @@ int launch_stream(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int
   return launch_status("w8a8_fp8_gemm");
 }
 
+// ================================================================== wide tiles
+// Many tokens: the tensor cores set the pace. A pair of CTAs (cta_group::2) owns a tile
+// of 256 tokens x BN weight rows: each CTA loads its 128 token rows and BN / 2 of the
+// weight rows per K block, half of what two single tiles would read, and folds the
+// sums of its own 128 tokens. Persistent, one pair per two SMs, tiles with the tokens
+// fastest so that the pairs at work share weight rows in L2.
+// Warp 0 loads, warp 1 issues (rank 0 only), warps 4-11 fold: two threads per token
+// row, BN / 2 columns each, in registers that setmaxnreg moves to them. A thread's
+// columns lie in one weight block, so a K block costs it one scale.
+// The fold of 128 x 256 sums is 64 packed multiply-adds per thread and K block, half
+// the time of the block's MMAs; two accumulators in tensor memory keep both going, and
+// what counts is how soon one is handed back. Measured at 4,096 x 34,816 x 5,120:
+// 1.52 ms at first; 0.79 with the hand-back a release of CTA scope (cluster scope waits
+// for global loads); 0.66 with the issuing warp kept converged; 0.59 without the abort
+// flag and the divisions in the folding loop (2,460 TFLOP/s; torch._scaled_mm without
+// block scales 0.51 on the same GPU, both under the power cap). Rows leave through
+// shared memory and TMA.
+// A role that gives up a wait does not tell the others within the loop: their own
+// bounded waits end theirs.
+constexpr int kWideConsumers = 8, kWideThreads = (4 + kWideConsumers) * 32;
+
+// (a0, a1) += (r0, r1) * f, both products in one instruction. Volatile, so that it stays
+// between the loads of tensor memory it is written between.
+__device__ __forceinline__ void fold2(float& a0, float& a1, uint32_t r0, uint32_t r1, uint64_t f2) {
+  asm volatile(
+      "{\n\t.reg .b64 a, r;\n\t"
+      "mov.b64 a, {%0, %1};\n\tmov.b64 r, {%2, %3};\n\t"
+      "fma.rn.f32x2 a, r, %4, a;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "r"(r0), "r"(r1), "l"(f2));
+}
+
+template <int BN>
+struct WideLayout {
+  static constexpr int kABytes = 128 * kBlk, kBBytes = BN / 2 * kBlk;   // per CTA
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = (192 * 1024) / kStageBytes;
+  static constexpr int kAcc = 512 / BN;
+  static constexpr int kOutBytes = kWideConsumers * 32 * 128;          // 32 rows x 128 bytes per warp
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kOutBytes;
+  static_assert(kSmem <= 227 * 1024 - 512, "shared memory of a CTA");
+};
+
+template <int BN>
+__global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
+    const Fp8GemmArgs p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+    const __grid_constant__ CUtensorMap map_o) {
+  pdl_enter();
+  using L = WideLayout<BN>;
+  constexpr int S = L::kStages, NA = L::kAcc, NC = BN / (kWideConsumers / 4);
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full_bar[S], done_bar[S], tempty_bar[NA], drain_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int s_abort;
+
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int rank = int(cluster::rank());
+  const int pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
+  const int m_tiles = (p.M + 255) / 256, total = m_tiles * p.n_tiles;   // n_tiles of BN rows
+  int armed = 0;
+
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&full_bar[i], 1), mbar_init(&done_bar[i], 1);
+    for (int i = 0; i < NA; ++i) mbar_init(&tempty_bar[i], 2 * kWideConsumers);
+    mbar_init(&drain_bar, 1);
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_pair(&tmem_slot, 512);
+  tc_fence_before_sync();
+  cluster::sync();   // both CTAs' barriers exist before either is signalled from the other
+  tc_fence_after_sync();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0), ring_s = smem_u32(ring);
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      const bool one = elect_one();
+      if (one) tma::prefetch_map(&map_w), tma::prefetch_map(&map_a);
+      const uint32_t full0 = cluster::map_shared(smem_u32(&full_bar[0]), 0);
+      bool ok = true;
+      int t = 0, s = 0;
+      uint32_t ph = 1;
+      for (int item = pair; item < total && ok; item += pairs) {
+        const int nt = item / m_tiles, mt = item - nt * m_tiles;
+        for (int kb = 0; kb < p.nkb; ++kb) {
+          ok = mbar_wait_warp(&done_bar[s], ph);
+          if (!ok) break;
+          if (one) {
+            const uint32_t st = ring_s + s * L::kStageBytes;
+            if (rank == 0) tma::mbar_expect_tx(&full_bar[s], 2 * L::kStageBytes);   // both CTAs' bytes
+            tma::load_2d_pair(st, &map_a, kb * kBlk, mt * 256 + rank * 128, full0 + s * 8);
+            tma::load_2d_pair(st + L::kABytes, &map_w, kb * kBlk, nt * BN + rank * (BN / 2), full0 + s * 8);
+          }
+          __syncwarp();
+          ++t;
+          if (++s == S) s = 0, ph ^= 1;
+        }
+      }
+      armed = t;
+      if (!ok && lane == 0) atomicExch(p.status, 1), s_abort = 1;
+    } else if (warp == 1 && rank == 0) {
+      constexpr uint32_t idesc = instr_desc(D_F32, 0, 0, 256, BN);
+      const uint32_t a_lo0 = smem_desc_lo(ring_s);
+      const bool one = elect_one();
+      bool ok = true;
+      int s = 0, b = 0;
+      uint32_t ph = 0, aph = 1;
+      for (int item = pair; item < total && ok; item += pairs) {
+        for (int kb = 0; kb < p.nkb; ++kb) {
+          ok = mbar_wait_warp(&tempty_bar[b], aph) && mbar_wait_warp(&full_bar[s], ph);
+          if (!ok) break;
+          tc_fence_after_sync();
+          if (one) {
+            const uint32_t a_lo = a_lo0 + s * (L::kStageBytes >> 4), b_lo = a_lo + (L::kABytes >> 4);
+            const uint32_t d = tmem + b * BN;
+            mma_f8_pair<false>(d, a_lo, b_lo, idesc);
+            mma_f8_pair<true>(d, a_lo + 2, b_lo + 2, idesc);
+            mma_f8_pair<true>(d, a_lo + 4, b_lo + 4, idesc);
+            mma_f8_pair<true>(d, a_lo + 6, b_lo + 6, idesc);
+            mma_commit_pair(&done_bar[s]);   // frees the stage and publishes the sums, in both CTAs
+          }
+          __syncwarp();
+          if (++s == S) s = 0, ph ^= 1;
+          if (++b == NA) b = 0, aph ^= 1;
+        }
+      }
+      if (!ok && lane == 0) atomicExch(p.status, 1), s_abort = 1;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int trow = (warp & 3) * 32 + lane;          // TMEM lane = token of this CTA's 128
+    const int cg = (warp - 4) >> 2;                   // which half of the BN columns
+    const uint32_t src0 = tmem + (uint32_t((warp & 3) * 32) << 16) + cg * NC;
+    const uint32_t tempty0 = cluster::map_shared(smem_u32(&tempty_bar[0]), 0);
+    int s = 0, b = 0;
+    uint32_t ph = 0;
+    bool dead = false;
+    for (int item = pair; item < total && !dead; item += pairs) {
+      const int nt = item / m_tiles, mt = item - nt * m_tiles;
+      const int m = mt * 256 + rank * 128 + trow, n0 = nt * BN + cg * NC;
+      const bool m_ok = m < p.M;
+      // rows and blocks past the edge read the last valid scale; their sums are not stored
+      const float* sa = p.sa + int64_t(m_ok ? m : p.M - 1) * p.sa_sm;
+      const float* sw = p.sw + int64_t((n0 < p.N ? n0 : p.N - 1) / kBlk) * p.sw_sn;
+      float a_next = __ldg(sa), w_next = __ldg(sw);
+      float acc[NC];
+#pragma unroll
+      for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+      for (int kb = 0; kb < p.nkb; ++kb) {
+        const float f = a_next * w_next;
+        uint64_t f2;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(f2) : "f"(f));
+        if (kb + 1 < p.nkb) {
+          sa += p.sa_sk, sw += p.sw_sk;
+          a_next = __ldg(sa), w_next = __ldg(sw);
+        }
+        if (!mbar_wait_warp(&done_bar[s], ph)) {
+          dead = true;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t src = src0 + b * BN;
+        constexpr int CH = 32;
+        uint32_t r[2][CH];
+        tmem_ld_32x32(src, r[0]);
+#pragma unroll
+        for (int c = 0; c < NC / CH; ++c) {
+          tmem_ld_wait();
+          if (c + 1 < NC / CH) {
+            tmem_ld_32x32(src + (c + 1) * CH, r[(c + 1) & 1]);
+          } else {   // everything read: the accumulator may be written again
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(tempty0 + b * 8);
+          }
+#pragma unroll
+          for (int j = 0; j < CH; j += 2) {
+            fold2(acc[c * CH + j], acc[c * CH + j + 1], r[c & 1][j], r[c & 1][j + 1], f2);
+          }
+        }
+        if (++s == S) s = 0, ph ^= 1;
+        if (++b == NA) b = 0;
+      }
+      if (dead) break;
+      if (p.bias != nullptr) {
+        // eight at a time: the whole row's loads in flight would cost its registers
+#pragma unroll
+        for (int j = 0; j < NC; j += 8) {
+#pragma unroll
+          for (int i = j; i < j + 8; ++i)
+            if (n0 + i < p.N) acc[i] += load_bias(p.bias, p.out_kind, n0 + i);
+          asm volatile("" ::: "memory");
+        }
+      }
+      if (p.tma_out) {
+        // 128 bytes of each of the warp's 32 rows at a time through shared memory, in the
+        // 128-byte swizzle (eight lanes write eight different chunks), out by TMA, which
+        // leaves out what lies past M or N
+        const uint32_t stage = ring_s + S * L::kStageBytes + (warp - 4) * (32 * 128);
+        const int row0 = mt * 256 + rank * 128 + (warp & 3) * 32;
+        auto put = [&](int chunk, uint4 v) {
+          *reinterpret_cast<uint4*>(ring + S * L::kStageBytes + (warp - 4) * (32 * 128) + sw128_offset(lane, chunk)) = v;
+        };
+        auto flush = [&](int col, int bytes) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0 && row0 < p.M && col < p.N) tma::store_2d(&map_o, stage, col * bytes, row0);
+          if (lane == 0) tma::store_commit();
+        };
+        auto reuse = [&] {
+          if (lane == 0) tma::store_wait_read<0>();
+          __syncwarp();
+        };
+        if (p.out_kind == kOutF32) {
+#pragma unroll
+          for (int j = 0; j < NC; j += 32) {
+            reuse();
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              put(c, make_uint4(__float_as_uint(acc[j + 4 * c]), __float_as_uint(acc[j + 4 * c + 1]),
+                                __float_as_uint(acc[j + 4 * c + 2]), __float_as_uint(acc[j + 4 * c + 3])));
+            flush(n0 + j, 4);
+          }
+        } else {
+          const bool bf = p.out_kind == kOutBf16;
+#pragma unroll
+          for (int j = 0; j < NC; j += 64) {
+            reuse();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float x = acc[j + 8 * c + 2 * i], y = acc[j + 8 * c + 2 * i + 1];
+                o[i] = bf ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+              }
+              put(c, make_uint4(o[0], o[1], o[2], o[3]));
+            }
+            flush(n0 + j, 2);
+          }
+        }
+      } else if (m_ok) {
+        const int64_t at = int64_t(m) * p.out_st + n0;
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          if (n0 + j < p.N) store_one(p.out, p.out_kind, at + j, acc[j]);
+      }
+    }
+    if (lane == 0) tma::store_wait_read<0>();   // the staged rows have left shared memory
+    if (dead) atomicExch(p.status, 1), s_abort = 1;
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (s_abort) {
+    // rank 0's barriers count the bytes of both CTAs and its thread issued all MMAs
+    if (rank == 0 && tid == 0) drain_armed_loads(full_bar, S, armed);
+    if (rank == 0 && warp == 1 && elect_one()) {
+      mma_commit_pair(&drain_bar);
+      mbar_wait(&drain_bar, 0);
+    }
+  }
+  tc_fence_before_sync();
+  cluster::sync();   // no signal of the other CTA is under way when this one ends
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+template <int BN>
+int launch_wide(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
+                int dev, cudaStream_t st) {
+  using L = WideLayout<BN>;
+  auto kernel = gemm_fp8_wide_kernel<BN>;
+  static bool done[64] = {};
+  if (!done[dev]) {
+    STRIX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
+    done[dev] = true;
+  }
+  p.n_tiles = (p.N + BN - 1) / BN;
+  const int64_t tiles = int64_t(p.n_tiles) * ((p.M + 255) / 256);
+  STRIX_CHECK(tiles < (int64_t(1) << 30), "matrix too large");
+  const int64_t bytes = p.out_kind == kOutF32 ? 4 : 2;
+  p.tma_out = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && (p.out_st * bytes) % 16 == 0;
+  CUtensorMap map_w, map_a, map_o = {};
+  STRIX_CHECK(tma::make_map_u8(&map_w, w, uint64_t(p.N), uint64_t(k), uint64_t(w_st), BN / 2) &&
+                  tma::make_map_u8(&map_a, a, uint64_t(p.M), uint64_t(k), uint64_t(a_st), 128) &&
+                  (!p.tma_out || tma::make_map_u8(&map_o, p.out, uint64_t(p.M), uint64_t(p.N) * bytes,
+                                                  uint64_t(p.M == 1 ? (p.N * bytes + 15) / 16 * 16 : p.out_st * bytes), 32)),
+              "tensor map encoding failed");
+  const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
+  STRIX_CUDA(cluster::launch(kernel, unsigned(2 * pairs), 2u, kWideThreads, L::kSmem, st, p, map_w, map_a, map_o));
+  return launch_status("w8a8_fp8_gemm");
+}
+
 // The checks that both entry points share; fills what the kernels read of the operands.
 int fp8_operands(Fp8GemmArgs& p, const void* a_q, const float* a_scale, const void* w, const float* w_scale,
                  int64_t m, int64_t n, int64_t k, int64_t& a_stride, int64_t& w_stride, int& dev, int& sms) {
@@ -317,7 +613,8 @@ int run_gemm(const Fp8GemmArgs& p, const void* a, int64_t a_st, const void* w, i
              int dev, cudaStream_t st) {
   if (p.M <= 16) return launch_stream<16>(p, a, a_st, w, w_st, k, sms, dev, st);
   if (p.M <= 32) return launch_stream<32>(p, a, a_st, w, w_st, k, sms, dev, st);
-  return launch_stream<64>(p, a, a_st, w, w_st, k, sms, dev, st);
+  if (p.M <= 64) return launch_stream<64>(p, a, a_st, w, w_st, k, sms, dev, st);
+  return launch_wide<256>(p, a, a_st, w, w_st, k, sms, dev, st);
 }
 
 }  // namespace

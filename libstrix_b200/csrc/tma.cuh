@@ -1,7 +1,7 @@
 // Tensor Memory Accelerator helpers for sm_100a: host-side tensor maps over
 // row matrices of bytes, device-side bulk tensor loads that complete on an
-// mbarrier. Loads only, never multicast; every load lands in the issuing CTA's
-// own shared memory.
+// mbarrier, and stores in bulk groups. Never multicast; every load lands in the
+// issuing CTA's own shared memory.
 //
 // A map describes a K-major matrix [rows, row_bytes] with a row stride, read in
 // boxes of `box_rows` rows x 128 bytes with the 128-byte swizzle, so a box lands
@@ -90,6 +90,18 @@ __device__ __forceinline__ void load_2d(uint32_t smem_dst, const CUtensorMap* ma
       : "memory");
 }
 
+// As load_2d for a CTA of a pair: the box lands in this CTA, the bytes complete the
+// barrier at `bar_cluster` (an address in the cluster's shared window, in either CTA
+// of the pair).
+__device__ __forceinline__ void load_2d_pair(uint32_t smem_dst, const CUtensorMap* map, int x, int y,
+                                             uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          smem_dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y)
+      : "memory");
+}
+
 __device__ __forceinline__ void load_4d(uint32_t smem_dst, const CUtensorMap* map, int c0, int c1,
                                         int c2, int c3, uint64_t* bar) {
   asm volatile(
@@ -98,6 +110,22 @@ __device__ __forceinline__ void load_4d(uint32_t smem_dst, const CUtensorMap* ma
       "l"(reinterpret_cast<uint64_t>(map)), "r"(umma::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
       "r"(c3)
       : "memory");
+}
+
+// Shared memory -> box at (byte x, row y), x a multiple of 16, y not negative; what
+// lies outside the matrix is not written. The writes of the generic proxy must have
+// been fenced (umma::fence_proxy_async). Completion is by the thread's bulk groups.
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, uint32_t smem_src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_src), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// All but the newest N groups of this thread have read their shared memory.
+template <int N>
+__device__ __forceinline__ void store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 
 // Asks the TMA to bring a box into L2 only: no shared memory, no barrier. Bytes

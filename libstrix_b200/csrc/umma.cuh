@@ -71,6 +71,26 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
+// One lane of a converged warp, the same one each time. The issuing warps stay converged
+// around it: tcgen05.mma and the TMA take their operands from the warp's uniform
+// registers, which the compiler computes them in only while it knows that all lanes run
+// together. Inside `if (lane == 0)` every operand crosses over from a thread's register
+// (measured: four MMAs of one K block 350 cycles in the issuing thread, longer than they
+// run at some tile sizes).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// mbar_wait by a whole warp, with one answer for all lanes.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
+}
+
 __device__ __forceinline__ void fence_mbar_init() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
@@ -285,6 +305,50 @@ __device__ __forceinline__ void mma_ss_lo(uint32_t tmem_d, uint32_t a_lo, uint32
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "n"(ACC ? 1 : 0)
         : "memory");
   }
+}
+
+// ----------------------------------------------------- pairs of CTAs (cta_group::2)
+// Two CTAs of a cluster share one MMA of M = 256: each holds its 128 rows of A, one
+// half of B's rows and the sums of its own rows. The CTA of rank 0 issues; tensor
+// memory is taken and given back by both.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
+               "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+
+// As mma_ss_lo<KIND_F8F6F4>, for the pair.
+template <bool ACC>
+__device__ __forceinline__ void mma_f8_pair(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+  const uint64_t adesc = desc_pack(a_lo, kDescHiSw128), bdesc = desc_pack(b_lo, kDescHiSw128);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "n"(ACC ? 1 : 0)
+      : "memory");
+}
+
+// Arrives on the barrier at this offset in BOTH CTAs once every MMA issued so far by
+// this thread has completed.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(uint16_t(3))
+      : "memory");
+}
+
+// Arrive on a barrier given by its address in the cluster's shared window. The release
+// is of CTA scope: what it hands over is tensor memory, ordered by the tcgen05 fences
+// around it, and a release of cluster scope waits for the thread's global loads too
+// (measured in the wide FP8 product: 1.52 against 0.79 ms).
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // Teardown after a bounded wait gave up (a role set the CTA's abort flag). A CTA
