@@ -13,9 +13,17 @@ from __future__ import annotations
 
 import torch
 
-from . import torch_ops  # noqa: F401  (registers torch.ops.strix.*)
+from . import torch_ops
 
 FP8 = torch.float8_e4m3fn
+
+
+def _eager(x) -> bool:
+    """Whether a call may go to the op's implementation without the dispatcher (4 us of
+    a call's 26, more than the smallest kernels run): an ordinary CUDA tensor outside a
+    trace. Anything else (fake tensors, subclasses, CPU tensors, torch.compile) takes
+    torch.ops.strix, with its shape inference and its errors."""
+    return type(x) is torch.Tensor and x.is_cuda and not torch.compiler.is_compiling()
 
 
 def _is_fp8(q_dtype: torch.dtype) -> bool:
@@ -32,28 +40,32 @@ def rms_norm_quant(x, weight, eps: float = 1e-6, residual=None, residual_out=Non
     itself for an update in place. The norm is taken of the fp32 sum, before that
     rounding. q_dtype float8_e4m3fn: scales fp32 [M, ceil(K / 128)], K a multiple of 16;
     int8: scales fp32 [M], K a multiple of 8."""
-    op = torch.ops.strix.rms_norm_quant_fp8 if _is_fp8(q_dtype) else torch.ops.strix.rms_norm_quant_token_i8
+    ns = torch_ops if _eager(x) else torch.ops.strix
+    op = ns.rms_norm_quant_fp8 if _is_fp8(q_dtype) else ns.rms_norm_quant_token_i8
     return op(x, weight, eps, residual, residual_out)
 
 
 def act_mul_quant(x, activation: str = "silu", q_dtype=FP8):
     """(q, scales) of act(x[:, :K]) * x[:, K:] for x [M, 2 K] (bf16, fp16 or fp32),
     activation silu or gelu_tanh; q and scales as rms_norm_quant returns them."""
-    op = torch.ops.strix.act_mul_quant_fp8 if _is_fp8(q_dtype) else torch.ops.strix.act_mul_quant_token_i8
+    ns = torch_ops if _eager(x) else torch.ops.strix
+    op = ns.act_mul_quant_fp8 if _is_fp8(q_dtype) else ns.act_mul_quant_token_i8
     return op(x, activation)
 
 
 def fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
     """[M, N] of a_q e4m3 [M, K] (a_scale fp32 [M, ceil(K / 128)]) and w e4m3 [N, K]
     (w_scale fp32 [ceil(N / 128), ceil(K / 128)]), K a multiple of 16."""
-    return torch.ops.strix.w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias, out_dtype)
+    ns = torch_ops if _eager(a_q) else torch.ops.strix
+    return ns.w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias, out_dtype)
 
 
 def fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation: str = "silu"):
     """(q e4m3 [M, N], scales) of act(gate) * up, where w e4m3 [2 N, K] holds the gate
     rows and then the up rows: fp8_gemm and act_mul_quant without the 16-bit rows
     between them."""
-    return torch.ops.strix.w8a8_fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation)
+    ns = torch_ops if _eager(a_q) else torch.ops.strix
+    return ns.w8a8_fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation)
 
 
 def fused_mlp_fp8_w8a8(x, norm_weight, w13, w13_scale, w2, w2_scale, eps: float = 1e-6, residual=None,

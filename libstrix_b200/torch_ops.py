@@ -1136,9 +1136,44 @@ def _groups(k: int) -> int:
     return (k + 127) // 128
 
 
-def _same_device(*tensors) -> None:
-    dev = tensors[0].device
-    _check(all(t is None or t.device == dev for t in tensors), "tensors must be on one device")
+def _same_device(first, *others) -> None:
+    dev = first.get_device()
+    for t in others:
+        _check(t is None or t.get_device() == dev, "tensors must be on one device")
+
+
+def _launch(t, entry: str, *args) -> None:
+    """Calls `entry` on t's device, its current stream the last argument. A decode step's
+    smallest kernels take less time than a call of Python's device and stream objects
+    (4.7 of a call's 26 us), hence the raw ones."""
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _after_tcgen05(t, op: str) -> None:
+    if _lib.CHECK_STATUS:
+        with torch.cuda.device(t.get_device()):
+            _lib.after_tcgen05(op)
+
+
+def _rows(like, m: int, k: int, dtype):
+    """An empty [m, k] on like's device (the cheapest factory call that names its strides)."""
+    return torch.empty_strided((m, k), (k, 1), dtype=dtype, device=like.device)
+
+
+def _quantised_rows(like, m: int, k: int, fp8: bool):
+    """Empty (q, scales) of the two 8-bit forms."""
+    new, dev = torch.empty_strided, like.device
+    if fp8:
+        g = (k + 127) // 128
+        return (new((m, k), (k, 1), dtype=torch.float8_e4m3fn, device=dev),
+                new((m, g), (g, 1), dtype=torch.float32, device=dev))
+    return (new((m, k), (k, 1), dtype=torch.int8, device=dev),
+            new((m,), (1,), dtype=torch.float32, device=dev))
 
 
 def _norm_fake(x, weight, eps, residual=None, residual_out=None):
@@ -1151,26 +1186,28 @@ def _norm_i8_fake(x, weight, eps, residual=None, residual_out=None):
 
 
 def _rms_norm_quant(x, weight, eps, residual, residual_out, fp8):
-    _check(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float16) and x.stride(1) == 1,
+    dtype = x.dtype
+    _check(x.dim() == 2 and (dtype is torch.bfloat16 or dtype is torch.float16) and x.stride(1) == 1,
            "x must be bf16 or fp16 [rows, K] with contiguous rows")
     m, k = x.shape
-    _check(k > 0 and k % (16 if fp8 else 8) == 0, f"K must be a multiple of {16 if fp8 else 8}")
-    _check(weight.dim() == 1 and weight.size(0) == k and weight.dtype in (x.dtype, torch.float32)
+    _check(k > 0 and k % (16 if fp8 else 8) == 0, "K must be a multiple of 16 (e4m3) or 8 (int8)")
+    _check(weight.shape == (k,) and (weight.dtype is dtype or weight.dtype is torch.float32)
            and weight.stride(0) == 1, "weight must be contiguous [K], of x's dtype or fp32")
     _check(eps >= 0, "eps must not be negative")
-    _check(residual_out is None or residual is not None, "residual_out needs a residual")
-    for name, t in (("residual", residual), ("residual_out", residual_out)):
-        _check(t is None or (t.dtype == x.dtype and t.shape == x.shape and t.stride(1) == 1),
-               f"{name} must match x")
+    if residual is not None:
+        _check(residual.dtype is dtype and residual.shape == x.shape and residual.stride(1) == 1,
+               "residual must match x")
+    if residual_out is not None:
+        _check(residual is not None, "residual_out needs a residual")
+        _check(residual_out.dtype is dtype and residual_out.shape == x.shape and residual_out.stride(1) == 1,
+               "residual_out must match x")
     _same_device(x, weight, residual, residual_out)
-    q = torch.empty((m, k), dtype=torch.float8_e4m3fn if fp8 else torch.int8, device=x.device)
-    s = torch.empty((m, _groups(k)) if fp8 else (m,), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.call("strix_rms_norm_quant", x.data_ptr(), _ptr(residual), _ptr(residual_out),
-                  weight.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0),
-                  0 if residual is None else residual.stride(0),
-                  0 if residual_out is None else residual_out.stride(0), k, s.stride(0), eps,
-                  int(x.dtype == torch.float16), int(weight.dtype == torch.float32), int(fp8), _stream())
+    q, s = _quantised_rows(x, m, k, fp8)
+    _launch(x, "strix_rms_norm_quant", x.data_ptr(), _ptr(residual), _ptr(residual_out),
+            weight.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0),
+            0 if residual is None else residual.stride(0),
+            0 if residual_out is None else residual_out.stride(0), k, _groups(k) if fp8 else 1, eps,
+            x.dtype == torch.float16, weight.dtype == torch.float32, fp8)
     return q, s
 
 
@@ -1204,15 +1241,14 @@ def _act_mul_i8_fake(x, activation="silu"):
 def _act_mul_quant(x, activation, fp8):
     _check(x.dim() == 2 and x.dtype in _OUT_KINDS and x.stride(1) == 1,
            "x must be bf16, fp16 or fp32 [rows, 2 K] with contiguous rows")
-    _check(activation in _ACTS, f"activation must be silu or gelu_tanh, got {activation}")
-    m, k = x.size(0), x.size(1) // 2
-    _check(x.size(1) % 2 == 0 and k > 0 and k % (16 if fp8 else 8) == 0,
-           f"K must be a multiple of {16 if fp8 else 8}")
-    q = torch.empty((m, k), dtype=torch.float8_e4m3fn if fp8 else torch.int8, device=x.device)
-    s = torch.empty((m, _groups(k)) if fp8 else (m,), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.call("strix_act_mul_quant", x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0), k,
-                  s.stride(0), _ACTS[activation], _OUT_KINDS[x.dtype], int(fp8), _stream())
+    _check(activation in _ACTS, "activation must be silu or gelu_tanh")
+    m, k2 = x.shape
+    k = k2 // 2
+    _check(k2 % 2 == 0 and k > 0 and k % (16 if fp8 else 8) == 0,
+           "K must be a multiple of 16 (e4m3) or 8 (int8)")
+    q, s = _quantised_rows(x, m, k, fp8)
+    _launch(x, "strix_act_mul_quant", x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0), k,
+            _groups(k) if fp8 else 1, _ACTS[activation], _OUT_KINDS[x.dtype], fp8)
     return q, s
 
 
@@ -1237,9 +1273,9 @@ def _fp8_operands(a_q, a_scale, w, w_scale):
     m, k = a_q.shape
     n = w.size(0)
     _check(n > 0 and k > 0 and k % 16 == 0, "K must be a multiple of 16")
-    _check(a_scale.dtype == torch.float32 and tuple(a_scale.shape) == (m, _groups(k)),
+    _check(a_scale.dtype == torch.float32 and a_scale.shape == (m, _groups(k)),
            "a_scale must be fp32 [M, ceil(K/128)]")
-    _check(w_scale.dtype == torch.float32 and tuple(w_scale.shape) == (_groups(n), _groups(k)),
+    _check(w_scale.dtype == torch.float32 and w_scale.shape == (_groups(n), _groups(k)),
            "block scales must be fp32 [ceil(N/128), ceil(K/128)]")
     _same_device(a_q, a_scale, w, w_scale)
     return m, n, k
@@ -1259,15 +1295,14 @@ def w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=None):
     out_dtype = out_dtype or torch.bfloat16
     _check(out_dtype in _OUT_KINDS, "out_dtype must be bf16, fp16 or fp32")
     if bias is not None:
-        _check(bias.dtype == out_dtype and tuple(bias.shape) == (n,) and bias.stride(0) == 1,
+        _check(bias.dtype == out_dtype and bias.shape == (n,) and bias.stride(0) == 1,
                "bias must be contiguous [N] of the output's dtype")
         _same_device(a_q, bias)
-    out = torch.empty((m, n), dtype=out_dtype, device=a_q.device)
-    with torch.cuda.device(a_q.device):
-        _lib.call("strix_w8a8_fp8_gemm", out.data_ptr(), a_q.data_ptr(), a_scale.data_ptr(), w.data_ptr(),
-                  w_scale.data_ptr(), _ptr(bias), m, n, k, a_q.stride(0), w.stride(0), n,
-                  *a_scale.stride(), *w_scale.stride(), _OUT_KINDS[out_dtype], _stream())
-        _lib.after_tcgen05("w8a8_fp8_gemm")
+    out = _rows(a_q, m, n, out_dtype)
+    _launch(a_q, "strix_w8a8_fp8_gemm", out.data_ptr(), a_q.data_ptr(), a_scale.data_ptr(), w.data_ptr(),
+            w_scale.data_ptr(), _ptr(bias), m, n, k, a_q.stride(0), w.stride(0), n,
+            *a_scale.stride(), *w_scale.stride(), _OUT_KINDS[out_dtype])
+    _after_tcgen05(a_q, "w8a8_fp8_gemm")
     return out
 
 
@@ -1284,18 +1319,16 @@ def w8a8_fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation="silu"):
     gate rows, then the up rows; (q e4m3 [M, N], scales fp32 [M, ceil(N / 128)]) of
     act(gate) * up, taken from the fp32 sums without a 16-bit step in between."""
     m, n2, k = _fp8_operands(a_q, a_scale, w, w_scale)
-    _check(activation in _ACTS, f"activation must be silu or gelu_tanh, got {activation}")
+    _check(activation in _ACTS, "activation must be silu or gelu_tanh")
     n = n2 // 2
     _check(n2 % 32 == 0, "w must hold gate and up rows, a multiple of 16 each")
-    q = torch.empty((m, n), dtype=torch.float8_e4m3fn, device=a_q.device)
-    s = torch.empty((m, _groups(n)), dtype=torch.float32, device=a_q.device)
+    q, s = _quantised_rows(a_q, m, n, True)
     nbytes = _lib.load().strix_w8a8_fp8_gated_workspace(m, n, k)
-    with torch.cuda.device(a_q.device):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=a_q.device) if nbytes > 0 else None
-        _lib.call("strix_w8a8_fp8_gated", q.data_ptr(), s.data_ptr(), a_q.data_ptr(), a_scale.data_ptr(),
-                  w.data_ptr(), w_scale.data_ptr(), _ptr(ws), nbytes, m, n, k, a_q.stride(0), w.stride(0), n,
-                  s.stride(0), *a_scale.stride(), *w_scale.stride(), _ACTS[activation], _stream())
-        _lib.after_tcgen05("w8a8_fp8_gemm_act_mul_quant")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=a_q.device) if nbytes > 0 else None
+    _launch(a_q, "strix_w8a8_fp8_gated", q.data_ptr(), s.data_ptr(), a_q.data_ptr(), a_scale.data_ptr(),
+            w.data_ptr(), w_scale.data_ptr(), _ptr(ws), nbytes, m, n, k, a_q.stride(0), w.stride(0), n,
+            _groups(n), *a_scale.stride(), *w_scale.stride(), _ACTS[activation])
+    _after_tcgen05(a_q, "w8a8_fp8_gemm_act_mul_quant")
     return q, s
 
 
