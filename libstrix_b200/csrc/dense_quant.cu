@@ -24,8 +24,8 @@ using namespace quant8;
 
 constexpr int kMaxRowThreads = 1024;
 
-// Sum over the CTA, the same value in every thread. `scratch` holds 32 floats and is
-// free again after the next __syncthreads().
+// Sum over the CTA, the same value in every thread. `scratch` holds 32 floats; it may be
+// written again after the next __syncthreads() of the CTA.
 __device__ __forceinline__ float block_sum(float v, float* scratch) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -70,92 +70,115 @@ struct NormArgs {
   const void* w;                  // 16-bit as x, or fp32
   uint8_t* q;
   float* scales;
-  int64_t x_st, r_st, ro_st, q_st, s_st;
+  int64_t x_st, r_st, ro_st, q_st, s_st, rows;
   int k8;                         // vectors of eight per row
   float inv_k, eps;
 };
 
-// One CTA per row; thread t holds vectors t, t + T, ... (V of them) of the row. T is a
-// multiple of 32, so 16 consecutive lanes always hold one group of 128.
+// A CTA walks rows blockIdx.x, + gridDim.x, ...; thread t holds vectors t, t + T, ... (V
+// of them) of a row. T is a multiple of 32, so 16 consecutive lanes always hold one
+// group of 128. The next row's loads are issued as soon as this one's values are in
+// fp32 registers, and stay in flight through its reductions; the weights stay in
+// registers (as 16-bit pairs) for all rows. The sum may replace x or the residual in
+// place: no row is read by two CTAs, and a row is read before any of it is written.
 template <bool F8, bool F16, bool WF32, int V>
 __global__ void __launch_bounds__(kMaxRowThreads) rms_norm_quant_kernel(const NormArgs p) {
   pdl_enter();
-  __shared__ float s_sum[32], s_max[32];
-  const int64_t row = blockIdx.x;
+  __shared__ float s_sum[2][32], s_max[2][32];
+  constexpr bool kAhead = V <= 2;   // rows beyond 16,384 columns have no registers to spare for it
   const int tid = threadIdx.x, T = blockDim.x;
-  float v[V][8];
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = i * T + tid;
-    if (c >= p.k8) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      continue;
-    }
-    unpack8<F16>(*reinterpret_cast<const uint4*>(p.x + row * p.x_st + c * 8), v[i]);
-    if (p.residual != nullptr) {
-      float r[8];
-      unpack8<F16>(*reinterpret_cast<const uint4*>(p.residual + row * p.r_st + c * 8), r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] += r[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum += v[i][j] * v[i][j];
-  }
-  if (p.residual_out != nullptr) {
+  uint4 xr[V], rr[V], wr[V];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = i * T + tid;
+      xr[i] = rr[i] = make_uint4(0u, 0u, 0u, 0u);
       if (c >= p.k8) continue;
-      uint4 o;
-      if constexpr (F16)
-        o = make_uint4(pack_f16x2(v[i][0], v[i][1]), pack_f16x2(v[i][2], v[i][3]),
-                       pack_f16x2(v[i][4], v[i][5]), pack_f16x2(v[i][6], v[i][7]));
-      else
-        o = make_uint4(pack_bf16x2(v[i][0], v[i][1]), pack_bf16x2(v[i][2], v[i][3]),
-                       pack_bf16x2(v[i][4], v[i][5]), pack_bf16x2(v[i][6], v[i][7]));
-      *reinterpret_cast<uint4*>(p.residual_out + row * p.ro_st + c * 8) = o;
+      xr[i] = *reinterpret_cast<const uint4*>(p.x + row * p.x_st + c * 8);
+      if (p.residual != nullptr) rr[i] = *reinterpret_cast<const uint4*>(p.residual + row * p.r_st + c * 8);
     }
+  };
+  auto weights = [&](int c) {
+    return c < p.k8 ? __ldg(reinterpret_cast<const uint4*>(p.w) + c) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  if constexpr (kAhead) fetch(blockIdx.x);
+  if constexpr (!WF32 && kAhead) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) wr[i] = weights(i * T + tid);
   }
-  const float rstd = __frsqrt_rn(__fadd_rn(block_sum(sum, s_sum) * p.inv_k, p.eps));
-  float row_max = 0.f;
+  int par = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, par ^= 1) {
+    float v[V][8];
+    float sum = 0.f;
+    if constexpr (!kAhead) fetch(row);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = i * T + tid;
-    float w[8];
-    if (c >= p.k8) {
+    for (int i = 0; i < V; ++i) {
+      unpack8<F16>(xr[i], v[i]);
+      if (p.residual != nullptr) {
+        float r[8];
+        unpack8<F16>(rr[i], r);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = 0.f;
-    } else if constexpr (WF32) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p.w) + c * 2);
-      const float4 b = __ldg(reinterpret_cast<const float4*>(p.w) + c * 2 + 1);
-      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+        for (int j = 0; j < 8; ++j) v[i][j] += r[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += v[i][j] * v[i][j];
+    }
+    if (kAhead && row + gridDim.x < p.rows) fetch(row + gridDim.x);
+    if (p.residual_out != nullptr) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = i * T + tid;
+        if (c >= p.k8) continue;
+        uint4 o;
+        if constexpr (F16)
+          o = make_uint4(pack_f16x2(v[i][0], v[i][1]), pack_f16x2(v[i][2], v[i][3]),
+                         pack_f16x2(v[i][4], v[i][5]), pack_f16x2(v[i][6], v[i][7]));
+        else
+          o = make_uint4(pack_bf16x2(v[i][0], v[i][1]), pack_bf16x2(v[i][2], v[i][3]),
+                         pack_bf16x2(v[i][4], v[i][5]), pack_bf16x2(v[i][6], v[i][7]));
+        *reinterpret_cast<uint4*>(p.residual_out + row * p.ro_st + c * 8) = o;
+      }
+    }
+    const float rstd = __frsqrt_rn(__fadd_rn(block_sum(sum, s_sum[par]) * p.inv_k, p.eps));
+    float row_max = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = i * T + tid;
+      float w[8];
+      if constexpr (WF32) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (c < p.k8) {
+          a = __ldg(reinterpret_cast<const float4*>(p.w) + c * 2);
+          b = __ldg(reinterpret_cast<const float4*>(p.w) + c * 2 + 1);
+        }
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+      } else {
+        unpack8<F16>(kAhead ? wr[i] : weights(c), w);
+      }
+      // past the row's end: zeros, whatever rstd is (0 * inf would be a NaN)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = c < p.k8 ? v[i][j] * rstd * w[j] : 0.f;
+      if constexpr (!F8) row_max = max_nan(row_max, abs_max8(v[i]));
+    }
+    if constexpr (F8) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = i * T + tid;
+        const float s = scale_of(group_max(abs_max8(v[i])), kTopF8);
+        if (c >= p.k8) continue;
+        *reinterpret_cast<uint2*>(p.q + row * p.q_st + c * 8) = pack8<true>(v[i], __fdiv_rn(1.f, s));
+        if ((c & 15) == 0) p.scales[row * p.s_st + (c >> 4)] = s;
+      }
     } else {
-      unpack8<F16>(__ldg(reinterpret_cast<const uint4*>(p.w) + c), w);
-    }
+      const float s = scale_of(block_max(row_max, s_max[par]), kTopI8);
+      const float inv = __fdiv_rn(1.f, s);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = c < p.k8 ? v[i][j] * rstd * w[j] : 0.f;
-    if constexpr (!F8) row_max = max_nan(row_max, abs_max8(v[i]));
-  }
-  if constexpr (F8) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = i * T + tid;
-      const float s = scale_of(group_max(abs_max8(v[i])), kTopF8);
-      if (c >= p.k8) continue;
-      *reinterpret_cast<uint2*>(p.q + row * p.q_st + c * 8) = pack8<true>(v[i], __fdiv_rn(1.f, s));
-      if ((c & 15) == 0) p.scales[row * p.s_st + (c >> 4)] = s;
+      for (int i = 0; i < V; ++i) {
+        const int c = i * T + tid;
+        if (c < p.k8) *reinterpret_cast<uint2*>(p.q + row * p.q_st + c * 8) = pack8<false>(v[i], inv);
+      }
+      if (tid == 0) p.scales[row * p.s_st] = s;
     }
-  } else {
-    const float s = scale_of(block_max(row_max, s_max), kTopI8);
-    const float inv = __fdiv_rn(1.f, s);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = i * T + tid;
-      if (c < p.k8) *reinterpret_cast<uint2*>(p.q + row * p.q_st + c * 8) = pack8<false>(v[i], inv);
-    }
-    if (tid == 0) p.scales[row * p.s_st] = s;
   }
 }
 
@@ -179,32 +202,66 @@ __device__ __forceinline__ void load8(const void* base, int64_t elem, float (&v)
   }
 }
 
-template <int IN>
-__device__ __forceinline__ void gated8(const ActArgs& p, int64_t row, int c, float (&y)[8]) {
-  float u[8];
-  load8<IN>(p.x, row * p.x_st + c * 8, y);
-  load8<IN>(p.x, row * p.x_st + (p.k8 + c) * 8, u);
+// y[u] = act(gate) * up of vector c[u] of row[u], for the U vectors with c[u] < k8; all
+// loads are issued before the first is used.
+template <int IN, int U>
+__device__ __forceinline__ void gated8(const ActArgs& p, const int64_t (&row)[U], const int (&c)[U],
+                                       float (&y)[U][8]) {
+  if constexpr (IN == 2) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = gate(y[j], p.act) * u[j];
+    for (int u = 0; u < U; ++u) {
+      if (c[u] >= p.k8) continue;
+      float up[8];
+      load8<IN>(p.x, row[u] * p.x_st + c[u] * 8, y[u]);
+      load8<IN>(p.x, row[u] * p.x_st + (p.k8 + c[u]) * 8, up);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[u][j] = gate(y[u][j], p.act) * up[j];
+    }
+  } else {
+    uint4 g[U], h[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      g[u] = h[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (c[u] >= p.k8) continue;
+      const uint16_t* x = static_cast<const uint16_t*>(p.x) + row[u] * p.x_st;
+      g[u] = ldg_stream(x + c[u] * 8), h[u] = ldg_stream(x + (p.k8 + c[u]) * 8);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float up[8];
+      unpack8<IN == 1>(g[u], y[u]), unpack8<IN == 1>(h[u], up);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[u][j] = gate(y[u][j], p.act) * up[j];
+    }
+  }
 }
 
 // e4m3, a scale per 128 columns: a team of 16 lanes per (row, group), no exchange
-// beyond the team.
-template <int IN>
+// beyond the team. A team takes U groups, their loads first.
+template <int IN, int U>
 __global__ void __launch_bounds__(256) act_mul_quant_fp8_kernel(const ActArgs p) {
   pdl_enter();
   const int groups = (p.k8 + 15) >> 4, sub = threadIdx.x & 15;
-  const int64_t team = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 4;
-  const bool live = team < p.rows * groups;
-  const int64_t row = live ? team / groups : 0;
-  const int g = live ? int(team - row * groups) : 0, c = g * 16 + sub;
-  const bool have = live && c < p.k8;
-  float y[8] = {};
-  if (have) gated8<IN>(p, row, c, y);
-  const float s = scale_of(group_max(abs_max8(y)), kTopF8);
-  if (!have) return;
-  *reinterpret_cast<uint2*>(p.q + row * p.q_st + c * 8) = pack8<true>(y, __fdiv_rn(1.f, s));
-  if (sub == 0) p.scales[row * p.s_st + g] = s;
+  const int64_t total = p.rows * groups, team0 = int64_t(blockIdx.x) * (16 * U) + (threadIdx.x >> 4);
+  float y[U][8];
+  int64_t row[U];
+  int c[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t team = team0 + u * 16;
+    row[u] = team < total ? team / groups : 0;
+    c[u] = team < total ? int(team - row[u] * groups) * 16 + sub : p.k8;   // k8: nothing to do
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[u][j] = 0.f;
+  }
+  gated8<IN, U>(p, row, c, y);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float s = scale_of(group_max(abs_max8(y[u])), kTopF8);
+    if (c[u] >= p.k8) continue;
+    *reinterpret_cast<uint2*>(p.q + row[u] * p.q_st + c[u] * 8) = pack8<true>(y[u], __fdiv_rn(1.f, s));
+    if (sub == 0) p.scales[row[u] * p.s_st + (c[u] >> 4)] = s;
+  }
 }
 
 // int8, a scale per row: one CTA per row, the row in registers as in the norm.
@@ -215,37 +272,48 @@ __global__ void __launch_bounds__(kMaxRowThreads) act_mul_quant_token_kernel(con
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, T = blockDim.x;
   float y[V][8];
-  float m = 0.f;
+  int64_t rows[V];
+  int c[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = i * T + tid;
+    rows[i] = row, c[i] = i * T + tid;
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[i][j] = 0.f;
-    if (c < p.k8) gated8<IN>(p, row, c, y[i]);
-    m = max_nan(m, abs_max8(y[i]));
   }
+  gated8<IN, V>(p, rows, c, y);
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) m = max_nan(m, abs_max8(y[i]));
   const float s = scale_of(block_max(m, s_max), kTopI8);
   const float inv = __fdiv_rn(1.f, s);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = i * T + tid;
-    if (c < p.k8) *reinterpret_cast<uint2*>(p.q + row * p.q_st + c * 8) = pack8<false>(y[i], inv);
-  }
+  for (int i = 0; i < V; ++i)
+    if (c[i] < p.k8) *reinterpret_cast<uint2*>(p.q + row * p.q_st + c[i] * 8) = pack8<false>(y[i], inv);
   if (tid == 0) p.scales[row * p.s_st] = s;
 }
 
-// Threads and vectors per thread of a row kernel: the fewest vectors that hold the
-// row in at most 1,024 threads.
+// Threads and vectors per thread of a row kernel: the fewest vectors, and at least
+// v_min, that hold the row in at most 1,024 threads.
 struct RowShape {
   int threads, v;
 };
-RowShape row_shape(int64_t k8) {
-  int v = 1;
+RowShape row_shape(int64_t k8, int v_min) {
+  int v = v_min;
   while (v < 8 && k8 > int64_t(v) * kMaxRowThreads) v *= 2;
   return {int((k8 + v * 32 - 1) / (v * 32)) * 32, v};
 }
 
 constexpr int64_t kMaxRowK = 8 * 8 * kMaxRowThreads;
+
+// The current device and its multiprocessors (asked once per device).
+int device_sms(int& dev, int& sms) {
+  static int count[64] = {};
+  STRIX_CUDA(cudaGetDevice(&dev));
+  STRIX_CHECK(dev >= 0 && dev < 64, "device index %d out of range", dev);
+  if (!count[dev]) STRIX_CUDA(cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev));
+  sms = count[dev];
+  return STRIX_OK;
+}
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
@@ -255,24 +323,42 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
   return x < y + uintptr_t(b_bytes) && y < x + uintptr_t(a_bytes);
 }
 
-template <bool F8, bool F16, bool WF32>
-int launch_norm(const NormArgs& p, int64_t rows, cudaStream_t st) {
-  const RowShape s = row_shape(p.k8);
-  const unsigned grid = unsigned(rows);
-  if (s.v == 1) launch_chain(rms_norm_quant_kernel<F8, F16, WF32, 1>, grid, s.threads, 0, st, p);
-  else if (s.v == 2) launch_chain(rms_norm_quant_kernel<F8, F16, WF32, 2>, grid, s.threads, 0, st, p);
-  else if (s.v == 4) launch_chain(rms_norm_quant_kernel<F8, F16, WF32, 4>, grid, s.threads, 0, st, p);
-  else launch_chain(rms_norm_quant_kernel<F8, F16, WF32, 8>, grid, s.threads, 0, st, p);
+template <bool F8, bool F16, bool WF32, int V>
+int launch_norm_v(const NormArgs& p, int threads, int sms, int dev, cudaStream_t st) {
+  auto kernel = rms_norm_quant_kernel<F8, F16, WF32, V>;
+  // CTAs of this size that an SM holds at once (asked once per device and size)
+  static int resident[64][kMaxRowThreads / 32] = {};
+  int& per_sm = resident[dev][threads / 32 - 1];
+  if (per_sm == 0) STRIX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0));
+  STRIX_CHECK(per_sm > 0, "rms_norm_quant does not fit the device");
+  const int64_t slots = int64_t(sms) * per_sm;
+  launch_chain(kernel, unsigned(p.rows < slots ? p.rows : slots), threads, 0, st, p);
   return launch_status("rms_norm_quant");
+}
+
+template <bool F8, bool F16, bool WF32>
+int launch_norm(const NormArgs& p, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  const int rc = device_sms(dev, sms);
+  if (rc != STRIX_OK) return rc;
+  // one vector per thread where there are too few rows to fill the GPU (a row's time
+  // counts), two where there are many (bytes in flight count)
+  const RowShape s = row_shape(p.k8, p.rows > 2 * sms ? 2 : 1);
+  if (s.v == 1) return launch_norm_v<F8, F16, WF32, 1>(p, s.threads, sms, dev, st);
+  if (s.v == 2) return launch_norm_v<F8, F16, WF32, 2>(p, s.threads, sms, dev, st);
+  if (s.v == 4) return launch_norm_v<F8, F16, WF32, 4>(p, s.threads, sms, dev, st);
+  return launch_norm_v<F8, F16, WF32, 8>(p, s.threads, sms, dev, st);
 }
 
 template <int IN>
 int launch_act(const ActArgs& p, bool fp8, cudaStream_t st) {
   if (fp8) {
     const int64_t teams = p.rows * ((p.k8 + 15) / 16);
-    launch_chain(act_mul_quant_fp8_kernel<IN>, unsigned((teams + 15) / 16), 256, 0, st, p);
+    // two groups per team once there are more than four CTAs of one per SM
+    if (teams > 16 * 4 * 148) launch_chain(act_mul_quant_fp8_kernel<IN, 2>, unsigned((teams + 31) / 32), 256, 0, st, p);
+    else launch_chain(act_mul_quant_fp8_kernel<IN, 1>, unsigned((teams + 15) / 16), 256, 0, st, p);
   } else {
-    const RowShape s = row_shape(p.k8);
+    const RowShape s = row_shape(p.k8, 1);
     const unsigned grid = unsigned(p.rows);
     if (s.v == 1) launch_chain(act_mul_quant_token_kernel<IN, 1>, grid, s.threads, 0, st, p);
     else if (s.v == 2) launch_chain(act_mul_quant_token_kernel<IN, 2>, grid, s.threads, 0, st, p);
@@ -323,14 +409,14 @@ extern "C" int strix_rms_norm_quant(const void* x, const void* residual, void* r
   p.residual_out = static_cast<uint16_t*>(residual_out), p.w = weight;
   p.q = static_cast<uint8_t*>(q), p.scales = scales;
   p.x_st = x_stride, p.r_st = r_stride, p.ro_st = ro_stride, p.q_st = q_stride, p.s_st = s_stride;
-  p.k8 = int(k / 8), p.inv_k = float(1.0 / double(k)), p.eps = eps;
+  p.rows = rows, p.k8 = int(k / 8), p.inv_k = float(1.0 / double(k)), p.eps = eps;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (fp8) {
-    if (in_f16) return weight_f32 ? launch_norm<true, true, true>(p, rows, st) : launch_norm<true, true, false>(p, rows, st);
-    return weight_f32 ? launch_norm<true, false, true>(p, rows, st) : launch_norm<true, false, false>(p, rows, st);
+    if (in_f16) return weight_f32 ? launch_norm<true, true, true>(p, st) : launch_norm<true, true, false>(p, st);
+    return weight_f32 ? launch_norm<true, false, true>(p, st) : launch_norm<true, false, false>(p, st);
   }
-  if (in_f16) return weight_f32 ? launch_norm<false, true, true>(p, rows, st) : launch_norm<false, true, false>(p, rows, st);
-  return weight_f32 ? launch_norm<false, false, true>(p, rows, st) : launch_norm<false, false, false>(p, rows, st);
+  if (in_f16) return weight_f32 ? launch_norm<false, true, true>(p, st) : launch_norm<false, true, false>(p, st);
+  return weight_f32 ? launch_norm<false, false, true>(p, st) : launch_norm<false, false, false>(p, st);
 }
 
 extern "C" int strix_act_mul_quant(const void* x, void* q, float* scales, int64_t rows, int64_t k,

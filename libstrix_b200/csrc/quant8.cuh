@@ -34,10 +34,13 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
   return uint32_t(lo) | (uint32_t(hi) << 16);
 }
 
-__device__ __forceinline__ uint32_t pack_i8x4(float a, float b, float c, float d) {
-  const int qa = max(-127, min(127, __float2int_rn(a))), qb = max(-127, min(127, __float2int_rn(b)));
-  const int qc = max(-127, min(127, __float2int_rn(c))), qd = max(-127, min(127, __float2int_rn(d)));
-  return prmt(prmt(uint32_t(qa), uint32_t(qb), 0x0040), prmt(uint32_t(qc), uint32_t(qd), 0x0040), 0x5410);
+// Four values times inv, |product| at most 127 (and a last bit), as bytes. Added to 1.5 x
+// 2^23 the product rounds to a whole number, to nearest even, in the sum's low bits.
+__device__ __forceinline__ uint32_t pack_i8x4(float a, float b, float c, float d, float inv) {
+  constexpr float kMagic = 12582912.f;
+  const uint32_t qa = __float_as_uint(fmaf(a, inv, kMagic)), qb = __float_as_uint(fmaf(b, inv, kMagic));
+  const uint32_t qc = __float_as_uint(fmaf(c, inv, kMagic)), qd = __float_as_uint(fmaf(d, inv, kMagic));
+  return prmt(prmt(qa, qb, 0x0040), prmt(qc, qd, 0x0040), 0x5410);
 }
 
 template <bool F8>
@@ -46,8 +49,7 @@ __device__ __forceinline__ uint2 pack8(const float (&y)[8], float inv) {
     return make_uint2(pack_e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
                       pack_e4m3x4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv));
   else
-    return make_uint2(pack_i8x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
-                      pack_i8x4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv));
+    return make_uint2(pack_i8x4(y[0], y[1], y[2], y[3], inv), pack_i8x4(y[4], y[5], y[6], y[7], inv));
 }
 
 // Eight 16-bit values (bf16, or fp16) as fp32.
