@@ -57,13 +57,6 @@ __device__ __forceinline__ float group_max(float v) {
   return v;
 }
 
-__device__ __forceinline__ float abs_max8(const float (&y)[8]) {
-  float m = fabsf(y[0]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(y[i]));
-  return m;
-}
-
 struct NormArgs {
   const uint16_t *x, *residual;   // residual NULL: none
   uint16_t* residual_out;         // NULL: not stored; may be x or residual
@@ -166,12 +159,12 @@ __global__ void __launch_bounds__(kMaxRowThreads) rms_norm_quant_kernel(const No
         const int c = i * T + tid;
         const float s = scale_of(group_max(abs_max8(v[i])), kTopF8);
         if (c >= p.k8) continue;
-        *reinterpret_cast<uint2*>(p.q + row * p.q_st + c * 8) = pack8<true>(v[i], __fdiv_rn(1.f, s));
+        *reinterpret_cast<uint2*>(p.q + row * p.q_st + c * 8) = pack8<true>(v[i], rcp(s));
         if ((c & 15) == 0) p.scales[row * p.s_st + (c >> 4)] = s;
       }
     } else {
       const float s = scale_of(block_max(row_max, s_max[par]), kTopI8);
-      const float inv = __fdiv_rn(1.f, s);
+      const float inv = rcp(s);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int c = i * T + tid;
@@ -242,15 +235,18 @@ template <int IN, int U>
 __global__ void __launch_bounds__(256) act_mul_quant_fp8_kernel(const ActArgs p) {
   pdl_enter();
   const int groups = (p.k8 + 15) >> 4, sub = threadIdx.x & 15;
-  const int64_t total = p.rows * groups, team0 = int64_t(blockIdx.x) * (16 * U) + (threadIdx.x >> 4);
+  // 32 bits: the host refuses 2^31 groups, and a 64-bit division per team was a third of
+  // the kernel's instructions
+  const uint32_t total = uint32_t(p.rows) * uint32_t(groups);
+  const uint32_t team0 = blockIdx.x * uint32_t(16 * U) + (threadIdx.x >> 4);
   float y[U][8];
   int64_t row[U];
   int c[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t team = team0 + u * 16;
-    row[u] = team < total ? team / groups : 0;
-    c[u] = team < total ? int(team - row[u] * groups) * 16 + sub : p.k8;   // k8: nothing to do
+    const uint32_t team = team0 + u * 16, r = team / uint32_t(groups);
+    row[u] = team < total ? r : 0;
+    c[u] = team < total ? int(team - r * groups) * 16 + sub : p.k8;   // k8: nothing to do
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[u][j] = 0.f;
   }
@@ -259,7 +255,7 @@ __global__ void __launch_bounds__(256) act_mul_quant_fp8_kernel(const ActArgs p)
   for (int u = 0; u < U; ++u) {
     const float s = scale_of(group_max(abs_max8(y[u])), kTopF8);
     if (c[u] >= p.k8) continue;
-    *reinterpret_cast<uint2*>(p.q + row[u] * p.q_st + c[u] * 8) = pack8<true>(y[u], __fdiv_rn(1.f, s));
+    *reinterpret_cast<uint2*>(p.q + row[u] * p.q_st + c[u] * 8) = pack8<true>(y[u], rcp(s));
     if (sub == 0) p.scales[row[u] * p.s_st + (c[u] >> 4)] = s;
   }
 }
@@ -285,7 +281,7 @@ __global__ void __launch_bounds__(kMaxRowThreads) act_mul_quant_token_kernel(con
 #pragma unroll
   for (int i = 0; i < V; ++i) m = max_nan(m, abs_max8(y[i]));
   const float s = scale_of(block_max(m, s_max), kTopI8);
-  const float inv = __fdiv_rn(1.f, s);
+  const float inv = rcp(s);
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (c[i] < p.k8) *reinterpret_cast<uint2*>(p.q + row * p.q_st + c[i] * 8) = pack8<false>(y[i], inv);
@@ -428,7 +424,7 @@ extern "C" int strix_act_mul_quant(const void* x, void* q, float* scales, int64_
   STRIX_CHECK(k % (fp8 ? 16 : 8) == 0 && (fp8 ? k < (int64_t(1) << 30) : k <= kMaxRowK),
               "K must be a multiple of %d%s", fp8 ? 16 : 8, fp8 ? "" : ", at most 65536");
   if (rows == 0) return STRIX_OK;
-  STRIX_CHECK(rows < (int64_t(1) << 31) && rows * ((k + 127) / 128) < (int64_t(1) << 34), "too many rows");
+  STRIX_CHECK(rows < (int64_t(1) << 31) && rows * ((k + 127) / 128) < (int64_t(1) << 31) - 64, "too many rows");
   STRIX_CHECK(x != nullptr && q != nullptr && scales != nullptr, "pointers must not be NULL");
   STRIX_CHECK(aligned(x, 16) && aligned(q, 8) && x_stride % (in_type == 2 ? 4 : 8) == 0 && q_stride % 8 == 0,
               "16-byte aligned rows required");

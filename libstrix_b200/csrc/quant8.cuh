@@ -3,7 +3,7 @@
 //
 //   scale = amax / top (448 for e4m3, 127 for int8), 1 where that is below the
 //           smallest normal number (an all-zero group, or one too small to scale);
-//   q     = round(y * (1 / scale)) to the nearest value, ties to even.
+//   q     = y * (1 / scale) rounded to the nearest value, ties to even.
 // A NaN in a group makes its scale NaN, an infinity makes it infinite, so that
 // neither disappears in the bytes (max.NaN below; a plain fmaxf drops NaN).
 #pragma once
@@ -19,11 +19,31 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ float abs_max8(const float (&y)[8]) {
+  const float a = max_nan(fabsf(y[0]), fabsf(y[1]), fabsf(y[2])), b = max_nan(fabsf(y[3]), fabsf(y[4]), fabsf(y[5]));
+  return max_nan(max_nan(a, b), fabsf(y[6]), fabsf(y[7]));
+}
+
+__device__ __forceinline__ float rcp(float x) {   // within a step of fp32
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 constexpr float kTopF8 = 448.f, kTopI8 = 127.f;
 constexpr float kSmallestNormal = 1.17549435e-38f;
 
+// amax / TOP, as a product with the constant's reciprocal: a step or two of fp32 off the
+// quotient, which the values are then divided by (an IEEE division in each of a group's 16
+// lanes costs a tenth of act_mul_quant's instructions).
 __device__ __forceinline__ float scale_of(float amax, float top) {
-  const float s = __fdiv_rn(amax, top);
+  const float s = amax * (1.f / top);
   return s < kSmallestNormal ? 1.f : s;   // NaN compares false and stays
 }
 
@@ -72,7 +92,7 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
 // through one exponential: a tanh under fast-math holds 11 bits only.
 __device__ __forceinline__ float gate(float g, int act) {
   const float u = act == 1 ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-  return __fdividef(g, 1.f + __expf(-u));
+  return g * rcp(1.f + __expf(-u));
 }
 
 }  // namespace quant8
