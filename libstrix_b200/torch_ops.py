@@ -1160,13 +1160,8 @@ def _after_tcgen05(t, op: str) -> None:
             _lib.after_tcgen05(op)
 
 
-def _rows(like, m: int, k: int, dtype):
-    """An empty [m, k] on like's device (the cheapest factory call that names its strides)."""
-    return torch.empty_strided((m, k), (k, 1), dtype=dtype, device=like.device)
-
-
 def _quantised_rows(like, m: int, k: int, fp8: bool):
-    """Empty (q, scales) of the two 8-bit forms."""
+    """Empty (q, scales) of the two 8-bit forms (empty_strided: the cheapest factory call)."""
     new, dev = torch.empty_strided, like.device
     if fp8:
         g = (k + 127) // 128
@@ -1186,28 +1181,32 @@ def _norm_i8_fake(x, weight, eps, residual=None, residual_out=None):
 
 
 def _rms_norm_quant(x, weight, eps, residual, residual_out, fp8):
-    dtype = x.dtype
-    _check(x.dim() == 2 and (dtype is torch.bfloat16 or dtype is torch.float16) and x.stride(1) == 1,
+    dtype, shape, x_st = x.dtype, x.shape, x.stride()
+    _check(len(shape) == 2 and (dtype is torch.bfloat16 or dtype is torch.float16) and x_st[1] == 1,
            "x must be bf16 or fp16 [rows, K] with contiguous rows")
-    m, k = x.shape
+    m, k = shape
     _check(k > 0 and k % (16 if fp8 else 8) == 0, "K must be a multiple of 16 (e4m3) or 8 (int8)")
-    _check(weight.shape == (k,) and (weight.dtype is dtype or weight.dtype is torch.float32)
-           and weight.stride(0) == 1, "weight must be contiguous [K], of x's dtype or fp32")
+    w_f32 = weight.dtype is torch.float32
+    _check(weight.shape == (k,) and (w_f32 or weight.dtype is dtype) and weight.stride() == (1,),
+           "weight must be contiguous [K], of x's dtype or fp32")
     _check(eps >= 0, "eps must not be negative")
+    r_ptr = ro_ptr = None
+    r_st = ro_st = 0
     if residual is not None:
-        _check(residual.dtype is dtype and residual.shape == x.shape and residual.stride(1) == 1,
-               "residual must match x")
+        r_st, one = residual.stride() if residual.dim() == 2 else (0, 0)
+        _check(one == 1 and residual.dtype is dtype and residual.shape == shape, "residual must match x")
+        r_ptr = residual.data_ptr()
     if residual_out is not None:
         _check(residual is not None, "residual_out needs a residual")
-        _check(residual_out.dtype is dtype and residual_out.shape == x.shape and residual_out.stride(1) == 1,
+        ro_st, one = residual_out.stride() if residual_out.dim() == 2 else (0, 0)
+        _check(one == 1 and residual_out.dtype is dtype and residual_out.shape == shape,
                "residual_out must match x")
+        ro_ptr = residual_out.data_ptr()
     _same_device(x, weight, residual, residual_out)
     q, s = _quantised_rows(x, m, k, fp8)
-    _launch(x, "strix_rms_norm_quant", x.data_ptr(), _ptr(residual), _ptr(residual_out),
-            weight.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0),
-            0 if residual is None else residual.stride(0),
-            0 if residual_out is None else residual_out.stride(0), k, _groups(k) if fp8 else 1, eps,
-            x.dtype == torch.float16, weight.dtype == torch.float32, fp8)
+    _launch(x, "strix_rms_norm_quant", x.data_ptr(), r_ptr, ro_ptr, weight.data_ptr(), q.data_ptr(),
+            s.data_ptr(), m, k, x_st[0], r_st, ro_st, k, (k + 127) // 128 if fp8 else 1, eps,
+            dtype is torch.float16, w_f32, fp8)
     return q, s
 
 
@@ -1239,16 +1238,17 @@ def _act_mul_i8_fake(x, activation="silu"):
 
 
 def _act_mul_quant(x, activation, fp8):
-    _check(x.dim() == 2 and x.dtype in _OUT_KINDS and x.stride(1) == 1,
+    shape, x_st, kind = x.shape, x.stride(), _OUT_KINDS.get(x.dtype)
+    _check(len(shape) == 2 and kind is not None and x_st[1] == 1,
            "x must be bf16, fp16 or fp32 [rows, 2 K] with contiguous rows")
     _check(activation in _ACTS, "activation must be silu or gelu_tanh")
-    m, k2 = x.shape
+    m, k2 = shape
     k = k2 // 2
     _check(k2 % 2 == 0 and k > 0 and k % (16 if fp8 else 8) == 0,
            "K must be a multiple of 16 (e4m3) or 8 (int8)")
     q, s = _quantised_rows(x, m, k, fp8)
-    _launch(x, "strix_act_mul_quant", x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x.stride(0), k,
-            _groups(k) if fp8 else 1, _ACTS[activation], _OUT_KINDS[x.dtype], fp8)
+    _launch(x, "strix_act_mul_quant", x.data_ptr(), q.data_ptr(), s.data_ptr(), m, k, x_st[0], k,
+            (k + 127) // 128 if fp8 else 1, _ACTS[activation], kind, fp8)
     return q, s
 
 
@@ -1266,19 +1266,21 @@ def act_mul_quant_token_i8(x, activation="silu"):
 
 
 def _fp8_operands(a_q, a_scale, w, w_scale):
-    f8 = torch.float8_e4m3fn
-    _check(a_q.dim() == 2 and w.dim() == 2 and a_q.dtype == f8 and w.dtype == f8
-           and a_q.size(1) == w.size(1) and a_q.stride(1) == 1 and w.stride(1) == 1,
+    """(m, n, k, row stride of a_q, row stride of w)."""
+    f8, f32 = torch.float8_e4m3fn, torch.float32
+    a_shape, w_shape, a_st, w_st = a_q.shape, w.shape, a_q.stride(), w.stride()
+    _check(len(a_shape) == 2 and len(w_shape) == 2 and a_q.dtype is f8 and w.dtype is f8
+           and a_shape[1] == w_shape[1] and a_st[1] == 1 and w_st[1] == 1,
            "a_q, w must be float8_e4m3fn [M, K], [N, K] with contiguous rows")
-    m, k = a_q.shape
-    n = w.size(0)
+    m, k = a_shape
+    n = w_shape[0]
     _check(n > 0 and k > 0 and k % 16 == 0, "K must be a multiple of 16")
-    _check(a_scale.dtype == torch.float32 and a_scale.shape == (m, _groups(k)),
-           "a_scale must be fp32 [M, ceil(K/128)]")
-    _check(w_scale.dtype == torch.float32 and w_scale.shape == (_groups(n), _groups(k)),
+    g = (k + 127) // 128
+    _check(a_scale.dtype is f32 and a_scale.shape == (m, g), "a_scale must be fp32 [M, ceil(K/128)]")
+    _check(w_scale.dtype is f32 and w_scale.shape == ((n + 127) // 128, g),
            "block scales must be fp32 [ceil(N/128), ceil(K/128)]")
     _same_device(a_q, a_scale, w, w_scale)
-    return m, n, k
+    return m, n, k, a_st[0], w_st[0]
 
 
 def _w8a8_fp8_fake(a_q, a_scale, w, w_scale, bias=None, out_dtype=None):
@@ -1291,17 +1293,19 @@ def w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=None):
     """out [M, N] (bf16, or out_dtype fp16 / fp32) of e4m3 activations with one fp32 scale
     per (row, 128 columns) and e4m3 weights with one per 128 x 128 block; bias [N] of the
     output's dtype."""
-    m, n, k = _fp8_operands(a_q, a_scale, w, w_scale)
+    m, n, k, a_st, w_st = _fp8_operands(a_q, a_scale, w, w_scale)
     out_dtype = out_dtype or torch.bfloat16
-    _check(out_dtype in _OUT_KINDS, "out_dtype must be bf16, fp16 or fp32")
+    kind = _OUT_KINDS.get(out_dtype)
+    _check(kind is not None, "out_dtype must be bf16, fp16 or fp32")
+    bias_ptr = None
     if bias is not None:
-        _check(bias.dtype == out_dtype and bias.shape == (n,) and bias.stride(0) == 1,
+        _check(bias.dtype is out_dtype and bias.shape == (n,) and bias.stride() == (1,),
                "bias must be contiguous [N] of the output's dtype")
         _same_device(a_q, bias)
-    out = _rows(a_q, m, n, out_dtype)
+        bias_ptr = bias.data_ptr()
+    out = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=a_q.device)
     _launch(a_q, "strix_w8a8_fp8_gemm", out.data_ptr(), a_q.data_ptr(), a_scale.data_ptr(), w.data_ptr(),
-            w_scale.data_ptr(), _ptr(bias), m, n, k, a_q.stride(0), w.stride(0), n,
-            *a_scale.stride(), *w_scale.stride(), _OUT_KINDS[out_dtype])
+            w_scale.data_ptr(), bias_ptr, m, n, k, a_st, w_st, n, *a_scale.stride(), *w_scale.stride(), kind)
     _after_tcgen05(a_q, "w8a8_fp8_gemm")
     return out
 
@@ -1318,7 +1322,7 @@ def w8a8_fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation="silu"):
     """The gate-up product that ends in the down product's input: w e4m3 [2 N, K] holds the
     gate rows, then the up rows; (q e4m3 [M, N], scales fp32 [M, ceil(N / 128)]) of
     act(gate) * up, taken from the fp32 sums without a 16-bit step in between."""
-    m, n2, k = _fp8_operands(a_q, a_scale, w, w_scale)
+    m, n2, k, a_st, w_st = _fp8_operands(a_q, a_scale, w, w_scale)
     _check(activation in _ACTS, "activation must be silu or gelu_tanh")
     n = n2 // 2
     _check(n2 % 32 == 0, "w must hold gate and up rows, a multiple of 16 each")
@@ -1326,7 +1330,7 @@ def w8a8_fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation="silu"):
     nbytes = _lib.load().strix_w8a8_fp8_gated_workspace(m, n, k)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=a_q.device) if nbytes > 0 else None
     _launch(a_q, "strix_w8a8_fp8_gated", q.data_ptr(), s.data_ptr(), a_q.data_ptr(), a_scale.data_ptr(),
-            w.data_ptr(), w_scale.data_ptr(), _ptr(ws), nbytes, m, n, k, a_q.stride(0), w.stride(0), n,
+            w.data_ptr(), w_scale.data_ptr(), _ptr(ws), nbytes, m, n, k, a_st, w_st, n,
             _groups(n), *a_scale.stride(), *w_scale.stride(), _ACTS[activation])
     _after_tcgen05(a_q, "w8a8_fp8_gemm_act_mul_quant")
     return q, s
