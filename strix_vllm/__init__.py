@@ -8,6 +8,7 @@ to CUDA compute capability 10.x and its hook points those of vLLM 0.22:
     int8    compressed-tensors W8A8 int8 linears    -> _POSSIBLE_INT8_KERNELS[CUDA]
     fp8     block-scaled / per-channel FP8 linears   -> _POSSIBLE_FP8_BLOCK_KERNELS,
                                                         _POSSIBLE_FP8_KERNELS
+            (W8A16; block-scaled layers as W8A8 with STRIX_ENABLE=fp8_w8a8)
     moe     FP8 block-scaled experts                 -> fused_moe.oracle.fp8 selector
     attn    int8_per_token_head / bf16 paged attention, KV-cache write
                                                      -> a registered attention backend

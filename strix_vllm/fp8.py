@@ -4,13 +4,18 @@ widened exactly inside the kernel (strix::fp8_skinny_gemm up to 8 rows,
 strix::fp8_wmma_gemm beyond). Follows the reference's kernels for the same
 layers (python/strix_vllm/fp8.py:121-262); its row padding and compute-unit
 hints are gfx1151 tuning and are not carried over.
+
+STRIX_ENABLE=fp8_w8a8 (opt-in: it changes the numerics, as the reference keeps 16-bit
+activations) runs block-scaled layers beyond 8 rows as W8A8: the activations are
+quantised to e4m3 per (row, 128 columns) and the product runs on tcgen05
+(strix::w8a8_fp8_gemm), where the W8A16 kernel is a weight stream.
 """
 
 from __future__ import annotations
 
 import torch
 
-from strix_vllm import disabled
+from strix_vllm import _env_names, disabled
 
 _BLOCK = 128
 _registered = False
@@ -26,13 +31,32 @@ def apply_fp8(x_2d: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     return out if bias is None else out + bias
 
 
+def w8a8_enabled() -> bool:
+    return "fp8_w8a8" in _env_names("STRIX_ENABLE") and not disabled("fp8_w8a8")
+
+
+def apply_fp8_w8a8(x_2d: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
+                   bias: torch.Tensor | None) -> torch.Tensor:
+    """apply_fp8 for 128 x 128 block scales with 8-bit activations beyond 8 rows (up to
+    there the weight stream sets the pace and the activations stay exact), and for the
+    widths that the W8A16 kernels do not take."""
+    x_2d = x_2d.contiguous()
+    if x_2d.size(0) <= 8 and w.size(0) % 16 == 0:
+        return apply_fp8(x_2d, w, scales, bias)
+    from libstrix_b200 import dense, moe
+
+    q, s = moe.act_quant_fp8(x_2d)
+    return dense.fp8_gemm(q, s, w, scales, None if bias is None else bias.contiguous(), torch.bfloat16)
+
+
 def _apply_fake(x_2d, w, scales, bias):
     return x_2d.new_empty((x_2d.size(0), w.size(0)))
 
 
-def _apply(x_2d, w, scales, bias):
-    fn = getattr(torch.ops.vllm, "strix_fp8_apply", None) if _registered else None
-    return (fn or apply_fp8)(x_2d, w, scales, bias)
+def _apply(x_2d, w, scales, bias, w8a8=False):
+    name, direct = ("strix_fp8_w8a8_apply", apply_fp8_w8a8) if w8a8 else ("strix_fp8_apply", apply_fp8)
+    fn = getattr(torch.ops.vllm, name, None) if _registered else None
+    return (fn or direct)(x_2d, w, scales, bias)
 
 
 def block_kernel_class():
@@ -42,8 +66,10 @@ def block_kernel_class():
     from vllm.model_executor.utils import replace_parameter
 
     class StrixFp8BlockScaledMMKernel(Fp8BlockScaledMMLinearKernel):
-        # W8A16: no dynamic activation quantisation in front of the GEMM
+        # no dynamic activation quantisation by vLLM in front of the GEMM: W8A16, or W8A8
+        # with this library's quantiser
         apply_input_quant = False
+        w8a8 = w8a8_enabled()
 
         @classmethod
         def is_supported(cls, compute_capability=None):
@@ -76,7 +102,7 @@ def block_kernel_class():
         def apply_weights(self, layer, x, bias=None, **kwargs):
             params = self._get_layer_params(layer)
             x_2d = x.reshape(-1, x.shape[-1])
-            out = _apply(x_2d, params.weight, params.block_scale, bias)
+            out = _apply(x_2d, params.weight, params.block_scale, bias, self.w8a8)
             return out.reshape(*x.shape[:-1], params.weight.size(0))
 
         def apply_block_scaled_mm(self, A, B, As, Bs):
@@ -149,6 +175,8 @@ def register() -> None:
     from vllm.utils.torch_utils import direct_register_custom_op
 
     direct_register_custom_op(op_name="strix_fp8_apply", op_func=apply_fp8, mutates_args=[],
+                              fake_impl=_apply_fake)
+    direct_register_custom_op(op_name="strix_fp8_w8a8_apply", op_func=apply_fp8_w8a8, mutates_args=[],
                               fake_impl=_apply_fake)
     _registered = True
     block = linear_kernels._POSSIBLE_FP8_BLOCK_KERNELS.setdefault(PlatformEnum.CUDA, [])

@@ -486,6 +486,27 @@ def test_mlp_captured_replayed_and_on_another_stream(t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 9, 200])
+def test_vllm_linear_with_8_bit_activations(m):
+    """The opt-in form of the block-scaled linear class: beyond 8 rows the activations are
+    e4m3, each off by 2^-4 of its value at most; the terms' signs are mixed, so a row's
+    error stays below that share of its norm."""
+    from strix_vllm import fp8
+
+    x, _, _ = norm_case(m, 640, torch.bfloat16, 30, False)
+    _, _, w, sw = gemm_case(1, 392, 640, 31)
+    bias = torch.randn(392, generator=gen(32)).bfloat16()
+    out = fp8.apply_fp8_w8a8(x.to(DEV), w.to(DEV), sw.to(DEV), bias.to(DEV)).double().cpu()
+    status_ok()
+    ref = O.fp8_gemm(x, torch.ones(m, 5), w, sw, bias)
+    assert ((out - ref).norm(dim=1) <= 2.0 ** -4 * ref.norm(dim=1)).all()
+    # few rows keep 16-bit activations where that kernel takes the width (multiples of 16)
+    w, sw, bias = w[:384].to(DEV), sw[:3].to(DEV), bias[:384].to(DEV)
+    few = fp8.apply_fp8_w8a8(x[:3].to(DEV), w, sw, bias)
+    assert torch.equal(few, fp8.apply_fp8(x[:3].to(DEV), w, sw, bias))
+
+
+@pytest.mark.gpu
 def test_results_do_not_change_from_run_to_run():
     for m, n, k in ((1, 512, 4096), (50, 1024, 2048), (600, 2048, 1024)):
         a, sa, w, sw = (t.to(DEV) for t in gemm_case(m, n, k, 9))
@@ -595,6 +616,17 @@ def test_act_refusals(over, message):
 def test_product_refusals(name, over, message):
     with pytest.raises(strix.StrixError, match=message):
         _call(name, **over)
+
+
+def test_vllm_form_is_opt_in(monkeypatch):
+    from strix_vllm import fp8
+
+    monkeypatch.delenv("STRIX_ENABLE", raising=False)
+    assert not fp8.w8a8_enabled()
+    monkeypatch.setenv("STRIX_ENABLE", "dense_w8, fp8_w8a8")
+    assert fp8.w8a8_enabled()
+    monkeypatch.setenv("STRIX_DISABLE", "fp8_w8a8")
+    assert not fp8.w8a8_enabled()
 
 
 def test_empty_calls_need_no_device():
