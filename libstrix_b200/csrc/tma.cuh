@@ -112,8 +112,9 @@ __device__ __forceinline__ void load_4d(uint32_t smem_dst, const CUtensorMap* ma
       : "memory");
 }
 
-// Shared memory -> box at (byte x, row y), x a multiple of 16, y not negative; what
-// lies outside the matrix is not written. The writes of the generic proxy must have
+// Shared memory -> box at (byte x, row y), x a multiple of 16, y not negative; rows and
+// whole 16-byte pieces outside the matrix are not written (a row whose length is no
+// multiple of 16 bytes is overrun to the next one). The writes of the generic proxy must have
 // been fenced (umma::fence_proxy_async). Completion is by the thread's bulk groups.
 __device__ __forceinline__ void store_2d(const CUtensorMap* map, uint32_t smem_src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(

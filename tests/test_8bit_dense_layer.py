@@ -111,8 +111,9 @@ def test_norm_with_fp32_weight_and_large_eps(dtype):
 
 @pytest.mark.gpu
 def test_norm_int8_takes_widths_off_16():
-    x, r, w = norm_case(4, 1000, torch.bfloat16, 4)
-    check_norm(x, r, w, 1e-5, torch.int8)
+    for m, k in ((4, 1000), (3, 8), (400, 24)):
+        x, r, w = norm_case(m, k, torch.bfloat16, 4)
+        check_norm(x, r, w, 1e-5, torch.int8)
 
 
 @pytest.mark.gpu
@@ -294,6 +295,49 @@ def test_gemm_ragged(m, n, k, out_dtype):
 @pytest.mark.parametrize("m,n,k", [(1, 34816, 5120), (16, 5120, 17408), (700, 2560, 5120), (1500, 1024, 2048)])
 def test_gemm_at_layer_widths(m, n, k):
     check_gemm(m, n, k, seed=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [(0, torch.bfloat16), (1, torch.float16), (2, torch.float32)])
+@pytest.mark.parametrize("m,n", [(1, 77), (40, 77), (70, 333), (300, 701)])
+def test_gemm_into_rows_of_a_wider_matrix(m, n, kind, dtype):
+    """The C entry with an output stride: rows on 16-byte boundaries (they leave by TMA in the
+    wide kernel) and off them; what lies beside the output stays as it was."""
+    k = 400
+    a, sa, w, sw = (t.to(DEV) for t in gemm_case(m, n, k, 14))
+    want = dense.fp8_gemm(a, sa, w, sw, out_dtype=dtype)
+    for width, first in ((n + 64 - n % 64 + 64, 16), (n + 37, 3)):
+        wide = torch.full((m + 2, width), -7.0, dtype=dtype, device=DEV)
+        out = wide[1:m + 1, first:first + n]
+        _lib.call("strix_w8a8_fp8_gemm", out.data_ptr(), a.data_ptr(), sa.data_ptr(), w.data_ptr(), sw.data_ptr(),
+                  None, m, n, k, k, k, width, *sa.stride(), *sw.stride(), kind,
+                  torch.cuda.current_stream().cuda_stream)
+        status_ok()
+        assert torch.equal(out, want)
+        rest = wide.clone()
+        rest[1:m + 1, first:first + n] = -7.0
+        assert (rest == -7.0).all()
+
+
+@pytest.mark.gpu
+def test_gated_product_into_rows_of_a_wider_matrix():
+    for m in (9, 200):
+        n, k = 256, 272
+        a, sa, w, sw = (t.to(DEV) for t in gemm_case(m, 2 * n, k, 15))
+        q, s = dense.fp8_gemm_act_mul_quant(a, sa, w, sw)
+        wide = torch.full((m + 2, n + 48), 9.0, device=DEV).to(F8)
+        wide_s = torch.full((m + 2, 5), -7.0, device=DEV)
+        nbytes = _lib.load().strix_w8a8_fp8_gated_workspace(m, n, k)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=DEV)
+        out, out_s = wide[1:m + 1, 16:16 + n], wide_s[1:m + 1, 1:3]
+        _lib.call("strix_w8a8_fp8_gated", out.data_ptr(), out_s.data_ptr(), a.data_ptr(), sa.data_ptr(), w.data_ptr(),
+                  sw.data_ptr(), ws.data_ptr(), nbytes, m, n, k, k, k, n + 48, 5, *sa.stride(), *sw.stride(), 1,
+                  torch.cuda.current_stream().cuda_stream)
+        status_ok()
+        assert torch.equal(out.view(torch.uint8), q.view(torch.uint8)) and torch.equal(out_s, s)
+        rest, rest_s = wide.float(), wide_s.clone()
+        rest[1:m + 1, 16:16 + n], rest_s[1:m + 1, 1:3] = 9.0, -7.0
+        assert (rest == 9.0).all() and (rest_s == -7.0).all()
 
 
 @pytest.mark.gpu
@@ -513,6 +557,43 @@ def test_results_do_not_change_from_run_to_run():
         first = dense.fp8_gemm(a, sa, w, sw, out_dtype=torch.float32)
         for _ in range(5):
             assert torch.equal(first, dense.fp8_gemm(a, sa, w, sw, out_dtype=torch.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [3, 200])
+def test_first_call_of_a_process_may_be_captured(t):
+    """Nothing of a first call (attributes, occupancy, addresses) disturbs a capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = f"""
+import torch
+from libstrix_b200 import dense
+f8 = torch.float8_e4m3fn
+x = torch.randn({t}, 256, device="cuda").bfloat16()
+nw = torch.ones(256, device="cuda").bfloat16()
+w13, w2 = torch.randn(512, 256, device="cuda").to(f8), torch.randn(256, 256, device="cuda").to(f8)
+s13, s2 = torch.rand(4, 2, device="cuda"), torch.rand(2, 2, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = dense.fused_mlp_fp8_w8a8(x, nw, w13, s13, w2, s2)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, dense.fused_mlp_fp8_w8a8(x, nw, w13, s13, w2, s2))
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=240, cwd=Path(__file__).resolve().parent.parent)
+
+
+@pytest.mark.gpu
+def test_a_tracer_sees_the_ops():
+    """Under a dispatch mode (a tracer's) the wrappers go through the dispatcher."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, _, w = norm_case(2, 256, torch.bfloat16, 40, False)
+    graph = make_fx(lambda a, b: dense.rms_norm_quant(a, b))(x.to(DEV), w.to(DEV))
+    assert any("rms_norm_quant_fp8" in str(n.target) for n in graph.graph.nodes)
 
 
 @pytest.mark.gpu
