@@ -56,5 +56,17 @@ inline cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned size, un
   return cudaLaunchKernelEx(&cfg, kernel, P(static_cast<A&&>(args))...);
 }
 
+// How many clusters of `size` CTAs the current device runs at once, at one CTA per SM.
+template <typename... P>
+inline cudaError_t places(int* out, void (*kernel)(P...), unsigned size, unsigned block, size_t smem) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(size * 64), cfg.blockDim = dim3(block), cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  return cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
+}
+
 }  // namespace cluster
 }  // namespace strix

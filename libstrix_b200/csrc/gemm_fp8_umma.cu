@@ -63,25 +63,33 @@ __device__ __forceinline__ void store_one(void* out, int kind, int64_t at, float
 // fills the GPU, the result does not depend on timing and no scratch is needed.
 // Warp 0 loads (TMA), warp 1 issues, warp 2 stages the tokens' scales, warps 4-7
 // fold. Two CTAs share an SM, so one's start and join hide behind the other's stream.
-constexpr int kStreamThreads = 256;
+//
+// GATED: a tile is 128 gate rows and the 128 up rows of the same outputs, two MMAs per
+// K step over the same tokens; warps 8-11 fold the up rows. The join leaves a thread with
+// both sums of an output, and the 128 threads of a token with one group of the 8-bit
+// form. One CTA per SM (its stages are twice as large).
+constexpr int kMaxSplits = 8;   // CTAs of a cluster
 
-template <int NB>
+template <int NB, bool GATED>
 struct StreamLayout {
-  static constexpr int kWBytes = 128 * kBlk, kTBytes = NB * kBlk;
+  static constexpr int kTiles = GATED ? 2 : 1;                     // of 128 weight rows
+  static constexpr int kCtas = GATED ? 1 : 2;                      // per SM
+  static constexpr int kFoldWarps = 4 * kTiles, kThreads = 128 + 32 * kFoldWarps;
+  static constexpr int kWBytes = kTiles * 128 * kBlk, kTBytes = NB * kBlk;
   static constexpr int kStageBytes = kWBytes + kTBytes;
-  static constexpr int kStages = (100 * 1024) / kStageBytes;
-  static constexpr int kAcc = 4;                                   // accumulators in tensor memory
-  static constexpr int kTmemCols = kAcc * NB < 32 ? 32 : kAcc * NB;
+  static constexpr int kStages = ((GATED ? 204 : 100) * 1024) / kStageBytes;
+  static constexpr int kAcc = 4;                                   // K blocks in tensor memory
+  static constexpr int kTmemCols = kAcc * kTiles * NB < 32 ? 32 : kAcc * kTiles * NB;
   static constexpr int kSmem = 1024 + kStages * (kStageBytes + NB * 4);
-  static_assert(kStages * kStageBytes >= NB * 128 * 4, "the join reuses the ring");
+  static_assert(kStages * kStageBytes >= kTiles * NB * 128 * 4, "the join reuses the ring");
 };
 
-template <int NB>
-__global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
+template <int NB, bool GATED>
+__global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayout<NB, GATED>::kCtas) gemm_fp8_stream_kernel(
     const Fp8GemmArgs p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a) {
   pdl_enter();
-  using L = StreamLayout<NB>;
-  constexpr int S = L::kStages, NA = L::kAcc;
+  using L = StreamLayout<NB, GATED>;
+  constexpr int S = L::kStages, NA = L::kAcc, T = L::kTiles;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   float* s_scale = reinterpret_cast<float*>(ring + S * L::kStageBytes);    // [S][NB]
@@ -100,9 +108,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&full_bar[i], 1), mbar_init(&done_bar[i], 1);
-      mbar_init(&sfull_bar[i], 32), mbar_init(&sempty_bar[i], 4);
+      mbar_init(&sfull_bar[i], 32), mbar_init(&sempty_bar[i], L::kFoldWarps);
     }
-    for (int i = 0; i < NA; ++i) mbar_init(&tempty_bar[i], 4);
+    for (int i = 0; i < NA; ++i) mbar_init(&tempty_bar[i], L::kFoldWarps);
     mbar_init(&drain_bar, 1);
     s_abort = 0;
     fence_mbar_init();
@@ -131,6 +139,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
         const uint32_t st = ring_s + s * L::kStageBytes;
         tma::mbar_expect_tx(&full_bar[s], L::kStageBytes);
         tma::load_2d(st, &map_w, (k0 + t) * kBlk, n0, &full_bar[s]);
+        if constexpr (GATED) tma::load_2d(st + 128 * kBlk, &map_w, (k0 + t) * kBlk, p.N / 2 + n0, &full_bar[s]);
         tma::load_2d(st + L::kWBytes, &map_a, (k0 + t) * kBlk, m0, &full_bar[s]);
       }
       __syncwarp();
@@ -151,11 +160,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
       tc_fence_after_sync();
       if (one) {
         const uint32_t w_lo = w_lo0 + s * (L::kStageBytes >> 4), t_lo = w_lo + (L::kWBytes >> 4);
-        const uint32_t d = tmem + b * NB;
-        mma_ss_lo<KIND_F8F6F4, false>(d, w_lo, t_lo, idesc);
-        mma_ss_lo<KIND_F8F6F4, true>(d, w_lo + 2, t_lo + 2, idesc);
-        mma_ss_lo<KIND_F8F6F4, true>(d, w_lo + 4, t_lo + 4, idesc);
-        mma_ss_lo<KIND_F8F6F4, true>(d, w_lo + 6, t_lo + 6, idesc);
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+          const uint32_t d = tmem + (b * T + i) * NB, w_i = w_lo + i * (128 * kBlk >> 4);
+          mma_ss_lo<KIND_F8F6F4, false>(d, w_i, t_lo, idesc);
+          mma_ss_lo<KIND_F8F6F4, true>(d, w_i + 2, t_lo + 2, idesc);
+          mma_ss_lo<KIND_F8F6F4, true>(d, w_i + 4, t_lo + 4, idesc);
+          mma_ss_lo<KIND_F8F6F4, true>(d, w_i + 6, t_lo + 6, idesc);
+        }
         mma_commit(&done_bar[s]);   // frees the stage and publishes the sums
       }
       __syncwarp();
@@ -186,7 +198,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
     if (dead && lane == 0) atomicExch(p.status, 1), s_abort = 1;
   } else if (warp >= 4) {
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-    const float* sw = p.sw + int64_t(n0 / kBlk) * p.sw_sn + int64_t(k0) * p.sw_sk;
+    const int part_of = (warp - 4) >> 2;   // GATED: 0 gate rows, 1 up rows
+    const float* sw = p.sw + int64_t((part_of * (p.N / 2) + n0) / kBlk) * p.sw_sn + int64_t(k0) * p.sw_sk;
     float w_next = nk > 0 ? __ldg(sw) : 0.f;
     bool dead = false;
     int s = 0, b = 0;
@@ -203,7 +216,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
 #pragma unroll
       for (int c = 0; c < NC; c += 16) {
         uint32_t r[16];
-        tmem_ld_32x16(tmem + lane_base + b * NB + c, r);
+        tmem_ld_32x16(tmem + lane_base + (b * T + part_of) * NB + c, r);
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
@@ -235,9 +248,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
 
   // thread r of warps 4-7 holds the sums of weight row n0 + r for the NB tokens
   const int row = (warp & 3) * 32 + lane, n = n0 + row;
-  const bool n_ok = n < p.N;
-  if (p.splits == 1) {
-    if (warp >= 4 && n_ok) {
+  if (!GATED && p.splits == 1) {
+    if (warp >= 4 && n < p.N) {
       const float bias = load_bias(p.bias, p.out_kind, n);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
@@ -246,53 +258,85 @@ __global__ void __launch_bounds__(kStreamThreads, 2) gemm_fp8_stream_kernel(
     return;
   }
   // the join: every CTA lays its partial tile [token][row] into its ring (whose copies and
-  // MMAs have ended), then sums the tokens rank, rank + splits, ... over the cluster
+  // MMAs have ended), then groups of 128 threads sum tokens over the cluster
   float* part = reinterpret_cast<float*>(ring);
   if (warp >= 4) {
+    float* mine = part + (GATED ? (warp - 4) >> 2 : 0) * (NB * 128);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) part[j * 128 + row] = acc[j];
+    for (int j = 0; j < NB; ++j) mine[j * 128 + row] = acc[j];
   }
   cluster::sync();
-  {
-    const int r = tid & 127, col = n0 + r;
+  constexpr int G = L::kThreads / 128;
+  const int grp = warp >> 2, col = n0 + row;
+  const uint32_t own = smem_u32(part) + row * 4;
+  auto joined = [&](int at) {   // the sum of float `at` x 128 + row over the cluster, in rank order
+    float v[kMaxSplits];   // all reads on their way before the first is added
+#pragma unroll
+    for (int c = 0; c < kMaxSplits; ++c)
+      v[c] = c < p.splits ? cluster::ld_shared_f32(cluster::map_shared(own + at * 512, c)) : 0.f;
+#pragma unroll
+    for (int c = 1; c < kMaxSplits; ++c) v[0] += v[c];
+    return v[0];
+  };
+  if constexpr (GATED) {
+    __shared__ float s_amax[2][G][4];
+    int par = 0;
+    // all threads take the same rounds: they meet at a barrier in each
+    for (int j0 = rank * G; j0 < NB && m0 + j0 < p.M; j0 += G * p.splits, par ^= 1) {
+      const int j = j0 + grp;
+      const bool live = j < NB && m0 + j < p.M;
+      float y = 0.f;
+      if (live) y = quant8::gate(joined(j), p.gate_act) * joined(NB + j);
+      float amax = fabsf(y);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) amax = quant8::max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (lane == 0) s_amax[par][grp][warp & 3] = amax;
+      __syncthreads();
+      const float* a4 = s_amax[par][grp];
+      const float sc = quant8::scale_of(quant8::max_nan(quant8::max_nan(a4[0], a4[1], a4[2]), a4[3]), quant8::kTopF8);
+      if (live) {
+        static_cast<uint8_t*>(p.out)[int64_t(m0 + j) * p.out_st + col] =
+            uint8_t(quant8::pack_e4m3x4(y * quant8::rcp(sc), 0.f, 0.f, 0.f));
+        if (row == 0) p.q_scales[int64_t(m0 + j) * p.qs_st + n0 / kBlk] = sc;
+      }
+    }
+  } else {
     const float bias = col < p.N ? load_bias(p.bias, p.out_kind, col) : 0.f;
-    const uint32_t own = smem_u32(part);
-    for (int j = rank * 2 + (tid >> 7); j < NB; j += 2 * p.splits) {
-      if (m0 + j >= p.M) break;
-      float v = 0.f;
-      for (int c = 0; c < p.splits; ++c) v += cluster::ld_shared_f32(cluster::map_shared(own + (j * 128 + r) * 4, c));
+    for (int j = rank * G + grp; j < NB && m0 + j < p.M; j += G * p.splits) {
+      const float v = joined(j);
       if (col < p.N) store_one(p.out, p.out_kind, int64_t(m0 + j) * p.out_st + col, v + bias);
     }
   }
   cluster::sync();   // nobody leaves while a peer still reads its shared memory
 }
 
-template <int NB>
+template <int NB, bool GATED>
 int launch_stream(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
                   int dev, cudaStream_t st) {
-  using L = StreamLayout<NB>;
-  auto kernel = gemm_fp8_stream_kernel<NB>;
-  static bool done[64] = {};
-  if (!done[dev]) {
+  using L = StreamLayout<NB, GATED>;
+  auto kernel = gemm_fp8_stream_kernel<NB, GATED>;
+  static int places[64][kMaxSplits + 1] = {};   // clusters of c CTAs that find an SM each (asked once)
+  if (!places[dev][1]) {
     STRIX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
-    done[dev] = true;
+    for (int c = kMaxSplits; c >= 1; --c)
+      STRIX_CUDA(cluster::places(&places[dev][c], kernel, unsigned(c), unsigned(L::kThreads), L::kSmem));
   }
-  p.n_tiles = (p.N + 127) / 128;
+  p.n_tiles = GATED ? p.N / 256 : (p.N + 127) / 128;
   const int64_t tiles = int64_t(p.n_tiles) * ((p.M + NB - 1) / NB);
-  // As many CTAs per tile as keep the grid within 1.7 CTAs per SM (the rest of the second
-  // slot covers for the SMs that a cluster cannot use) and leave each two K blocks; no
-  // seven, whose clusters pack badly. Measured on 16 x 5,120 x 17,408 (40 tiles): 36.8, 22.7,
-  // 20.0, 19.2, 18.7, 18.8, 25.8 and 23.1 us with 1 to 8; on 272 tiles 29.8 with one, 32.9 with two.
+  // As many CTAs per tile as leave each two K blocks and every cluster a place at once: a
+  // second round costs more than shorter CTAs give. Measured on 16 x 5,120 x 17,408 (40
+  // tiles; clusters of 6 are the largest that all fit): 36.8, 22.7, 20.0, 19.2, 18.7, 18.8,
+  // 25.8 and 23.1 us with 1 to 8; on 272 tiles 29.8 us with one, 32.9 with two.
   int splits = 1;
-  for (int c : {2, 3, 4, 5, 6, 8})
-    if (tiles * c * 10 <= 17 * sms && p.nkb >= 2 * c) splits = c;
+  for (int c = 2; c <= kMaxSplits; ++c)
+    if (tiles <= int64_t(places[dev][c]) * L::kCtas && p.nkb >= 2 * c) splits = c;
   p.splits = splits;
   STRIX_CHECK(tiles * splits < (int64_t(1) << 31), "matrix too large");
   CUtensorMap map_w, map_a;
   STRIX_CHECK(tma::make_map_u8(&map_w, w, uint64_t(p.N), uint64_t(k), uint64_t(w_st), 128) &&
                   tma::make_map_u8(&map_a, a, uint64_t(p.M), uint64_t(k), uint64_t(a_st), NB),
               "tensor map encoding failed");
-  STRIX_CUDA(cluster::launch(kernel, unsigned(tiles * splits), unsigned(splits), kStreamThreads, L::kSmem, st, p, map_w, map_a));
+  STRIX_CUDA(cluster::launch(kernel, unsigned(tiles * splits), unsigned(splits), L::kThreads, L::kSmem, st, p, map_w, map_a));
   return launch_status("w8a8_fp8_gemm");
 }
 
@@ -695,9 +739,9 @@ int fp8_operands(Fp8GemmArgs& p, const void* a_q, const float* a_scale, const vo
 
 int run_gemm(const Fp8GemmArgs& p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
              int dev, cudaStream_t st) {
-  if (p.M <= 16) return launch_stream<16>(p, a, a_st, w, w_st, k, sms, dev, st);
-  if (p.M <= 32) return launch_stream<32>(p, a, a_st, w, w_st, k, sms, dev, st);
-  if (p.M <= 64) return launch_stream<64>(p, a, a_st, w, w_st, k, sms, dev, st);
+  if (p.M <= 16) return launch_stream<16, false>(p, a, a_st, w, w_st, k, sms, dev, st);
+  if (p.M <= 32) return launch_stream<32, false>(p, a, a_st, w, w_st, k, sms, dev, st);
+  if (p.M <= 64) return launch_stream<64, false>(p, a, a_st, w, w_st, k, sms, dev, st);
   // Tiles of 256 x 128 while they all run at once: 0.72 of the time of one 256 x 256 tile
   // (768 x 2,048 x 2,048: 8.1 against 11.0 us), but a second round costs more than the
   // larger tile's one (512 x 5,120 x 5,120: 24.8 against 20.9 us).
@@ -728,13 +772,13 @@ extern "C" int strix_w8a8_fp8_gemm(void* out, const void* a_q, const float* a_sc
   return run_gemm(p, a_q, a_stride, w, w_stride, k, sms, dev, static_cast<cudaStream_t>(stream));
 }
 
-// Whether the gated product runs in one kernel: the wide tiles' epilogue. Otherwise (few
-// tokens, or gate and up rows that share a weight block) fp32 rows go through a workspace.
-static bool gated_in_one(int64_t m, int64_t n) { return m > 64 && n % 128 == 0; }
+// Whether the gated product runs in one kernel. Otherwise (gate and up rows that share a
+// weight block) fp32 rows go through a workspace.
+static bool gated_in_one(int64_t n) { return n % 128 == 0; }
 
 extern "C" int64_t strix_w8a8_fp8_gated_workspace(int64_t m, int64_t n, int64_t k) {
   if (m < 0 || n <= 0 || k <= 0 || m >= (int64_t(1) << 31) || n >= (int64_t(1) << 30)) return -1;
-  return gated_in_one(m, n) ? 0 : m * 2 * n * 4;
+  return gated_in_one(n) ? 0 : m * 2 * n * 4;
 }
 
 extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, const float* a_scale,
@@ -754,8 +798,10 @@ extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, con
   STRIX_CHECK(m == 1 || (q_stride >= n && s_stride >= (n + 127) / 128), "output rows must not overlap");
   p.sa_sm = sa_stride_m, p.sa_sk = sa_stride_k, p.sw_sn = sw_stride_n, p.sw_sk = sw_stride_k;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (gated_in_one(m, n)) {
+  if (gated_in_one(n)) {
     p.out = q, p.out_st = q_stride, p.q_scales = scales, p.qs_st = s_stride, p.gate_act = gate_act;
+    if (m <= 16) return launch_stream<16, true>(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
+    if (m <= 32) return launch_stream<32, true>(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
     return launch_wide<256, true>(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
   }
   const int64_t need = m * 2 * n * 4;
