@@ -33,6 +33,15 @@ __device__ __forceinline__ float ld_shared_f32(uint32_t cluster_addr) {
   return v;
 }
 
+__device__ __forceinline__ float4 ld_shared_f32x4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
+  return v;
+}
+
 // A launch of `grid` CTAs in clusters of `size` along x (1: none), chained to the
 // kernel before it like launch_chain (common.cuh).
 template <typename... P, typename... A>

@@ -357,6 +357,9 @@ int launch_stream(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int
 // flag and the divisions in the folding loop (2,460 TFLOP/s; torch._scaled_mm without
 // block scales 0.51 on the same GPU, both under the power cap). Rows leave through
 // shared memory and TMA.
+// Few tiles (65 to some hundred tokens): a cluster of up to four pairs shares one along K;
+// each lays its sums into its ring, and every CTA adds a share of the tokens over the
+// cluster, in the order of K.
 // A role that gives up a wait does not tell the others within the loop: their own
 // bounded waits end theirs.
 constexpr int kWideConsumers = 8, kWideThreads = (4 + kWideConsumers) * 32;
@@ -373,6 +376,8 @@ __device__ __forceinline__ void fold2(float& a0, float& a1, uint32_t r0, uint32_
       : "r"(r0), "r"(r1), "l"(f2));
 }
 
+constexpr int kMaxPairs = 4;   // pairs of CTAs that share a tile along K
+
 template <int BN>
 struct WideLayout {
   static constexpr int kABytes = 128 * kBlk, kBBytes = BN / 2 * kBlk;   // per CTA
@@ -381,6 +386,8 @@ struct WideLayout {
   static constexpr int kAcc = 512 / BN;
   static constexpr int kOutBytes = kWideConsumers * 32 * 128;          // 32 rows x 128 bytes per warp
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kOutBytes;
+  static constexpr int kPartRow = BN * 4 + 16;   // a token's partial sums; odd in 16 bytes: no bank conflicts
+  static_assert(128 * kPartRow <= kStages * kStageBytes, "the join reuses the ring");
   static_assert(kSmem <= 227 * 1024 - 512, "shared memory of a CTA");
 };
 
@@ -404,8 +411,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
   // GATED: [tile parity][half of the outputs][token], where the other form stages its rows
   float(*s_amax)[2][128] = reinterpret_cast<float(*)[2][128]>(ring + S * L::kStageBytes);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  const int rank = int(cluster::rank());
-  const int pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
+  const uint32_t crank = cluster::rank(), lead = crank & ~1u;   // lead: the CTA that issues for this pair
+  const int rank = int(crank & 1), kpart = int(crank >> 1);
+  const int pair = int(blockIdx.x) / (2 * p.splits), pairs = int(gridDim.x) / (2 * p.splits);
+  // K blocks [k0, k0 + nk) of this pair (all of them unless a cluster shares a tile along K)
+  const int base = p.nkb / p.splits, rem = p.nkb % p.splits;
+  const int nk = base + (kpart < rem ? 1 : 0), k0 = kpart * base + min(kpart, rem);
   const int m_tiles = (p.M + 255) / 256, total = m_tiles * p.n_tiles;   // n_tiles of BN rows
   int armed = 0;
 
@@ -428,13 +439,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
     if (warp == 0) {
       const bool one = elect_one();
       if (one) tma::prefetch_map(&map_w), tma::prefetch_map(&map_a);
-      const uint32_t full0 = cluster::map_shared(smem_u32(&full_bar[0]), 0);
+      const uint32_t full0 = cluster::map_shared(smem_u32(&full_bar[0]), lead);
       bool ok = true;
       int t = 0, s = 0;
       uint32_t ph = 1;
       for (int item = pair; item < total && ok; item += pairs) {
         const int nt = item / m_tiles, mt = item - nt * m_tiles;
-        for (int kb = 0; kb < p.nkb; ++kb) {
+        for (int kb = k0; kb < k0 + nk; ++kb) {
           ok = mbar_wait_warp(&done_bar[s], ph);
           if (!ok) break;
           if (one) {
@@ -464,7 +475,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
       int s = 0, b = 0;
       uint32_t ph = 0, aph = 1;
       for (int item = pair; item < total && ok; item += pairs) {
-        for (int kb = 0; kb < p.nkb; ++kb) {
+        for (int kb = 0; kb < nk; ++kb) {
           ok = mbar_wait_warp(&tempty_bar[b], aph) && mbar_wait_warp(&full_bar[s], ph);
           if (!ok) break;
           tc_fence_after_sync();
@@ -475,7 +486,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
             mma_f8_pair<true>(d, a_lo + 2, b_lo + 2, idesc);
             mma_f8_pair<true>(d, a_lo + 4, b_lo + 4, idesc);
             mma_f8_pair<true>(d, a_lo + 6, b_lo + 6, idesc);
-            mma_commit_pair(&done_bar[s]);   // frees the stage and publishes the sums, in both CTAs
+            mma_commit_pair(&done_bar[s], lead);   // frees the stage and publishes the sums, in both CTAs
           }
           __syncwarp();
           if (++s == S) s = 0, ph ^= 1;
@@ -484,12 +495,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
       }
       if (!ok && lane == 0) atomicExch(p.status, 1), s_abort = 1;
     }
+    if (p.splits > 1) cluster::sync();   // the folding warps' exchange of partial sums
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // 128 x 40 + 256 x this stays within the launch's 384 x 168; of the values that do, the
+    // ones at which the compiler spills nothing in the loop
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(GATED ? 176 : 232));
     const int trow = (warp & 3) * 32 + lane;          // TMEM lane = token of this CTA's 128
     const int cg = (warp - 4) >> 2;                   // which half of the BN columns
     const uint32_t src0 = tmem + (uint32_t((warp & 3) * 32) << 16) + cg * NC;
-    const uint32_t tempty0 = cluster::map_shared(smem_u32(&tempty_bar[0]), 0);
+    const uint32_t tempty0 = cluster::map_shared(smem_u32(&tempty_bar[0]), lead);
     int s = 0, b = 0;
     uint32_t ph = 0, xph = 0;
     bool dead = false;
@@ -498,20 +512,20 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
       const int m = mt * 256 + rank * 128 + trow, n0 = GATED ? nt * 128 : nt * BN + cg * NC;
       const bool m_ok = m < p.M;
       // rows and blocks past the edge read the last valid scale; their sums are not stored
-      const float* sa = p.sa + int64_t(m_ok ? m : p.M - 1) * p.sa_sm;
-      const float* sw = p.sw + int64_t((n0 < p.N ? n0 : p.N - 1) / kBlk) * p.sw_sn;
+      const float* sa = p.sa + int64_t(m_ok ? m : p.M - 1) * p.sa_sm + int64_t(k0) * p.sa_sk;
+      const float* sw = p.sw + int64_t((n0 < p.N ? n0 : p.N - 1) / kBlk) * p.sw_sn + int64_t(k0) * p.sw_sk;
       // GATED: the up rows' block, as far from the gate rows' as the halves are
       const int64_t up_block = GATED ? int64_t(p.N / 2 / kBlk) * p.sw_sn : 0;
       float a_next = __ldg(sa), w_next = __ldg(sw), u_next = GATED ? __ldg(sw + up_block) : 0.f;
       float acc[NC];
 #pragma unroll
       for (int j = 0; j < NC; ++j) acc[j] = 0.f;
-      for (int kb = 0; kb < p.nkb; ++kb) {
+      for (int kb = 0; kb < nk; ++kb) {
         const float f = a_next * w_next, fu = a_next * u_next;
         uint64_t f2, fu2;
         asm("mov.b64 %0, {%1, %1};" : "=l"(f2) : "f"(f));
         asm("mov.b64 %0, {%1, %1};" : "=l"(fu2) : "f"(fu));
-        if (kb + 1 < p.nkb) {
+        if (kb + 1 < nk) {
           sa += p.sa_sk, sw += p.sw_sk;
           a_next = __ldg(sa), w_next = __ldg(sw);
           if constexpr (GATED) u_next = __ldg(sw + up_block);
@@ -544,6 +558,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
         if (++b == NA) b = 0;
       }
       if (dead) break;
+      if (p.splits > 1) {
+        // the one tile of this cluster: the partial sums [token][column] into the ring, whose
+        // copies and MMAs have ended (the last K block's are the last)
+        float4* mine = reinterpret_cast<float4*>(ring + trow * L::kPartRow + cg * (NC * 4));
+#pragma unroll
+        for (int j = 0; j < NC; j += 4) mine[j >> 2] = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        break;
+      }
       if constexpr (GATED) {
         // outputs nt * 128 + cg * 64 + j: gate in acc[j], up in acc[64 + j]
 #pragma unroll
@@ -659,6 +681,88 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
         }
       }
     }
+    if (p.splits > 1) {
+      // tokens kpart, kpart + splits, ... of the pair's 128 per CTA, one warp per token, four
+      // neighbouring columns per lane, kRows tokens at a time: all their reads are under way
+      // before the first sum is used. The partial sums are added in the order of K.
+      cluster::sync();
+      constexpr int kRows = 4;
+      const int nt = pair / m_tiles, mt = pair - nt * m_tiles;
+      const uint32_t own = ring_s + lane * 16;
+      auto joined = [&](float4(&v)[kRows], int row, int at) {
+        float4 x[kMaxPairs][kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+          for (int c = 0; c < kMaxPairs; ++c) {
+            const int r = row + i * p.splits * kWideConsumers;
+            x[c][i] = c < p.splits && r < 128
+                          ? cluster::ld_shared_f32x4(cluster::map_shared(own + r * L::kPartRow + at, uint32_t(2 * c + rank)))
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          v[i] = x[0][i];
+#pragma unroll
+          for (int c = 1; c < kMaxPairs; ++c)
+            v[i].x += x[c][i].x, v[i].y += x[c][i].y, v[i].z += x[c][i].z, v[i].w += x[c][i].w;
+        }
+      };
+      const int m0 = mt * 256 + rank * 128;
+      for (int row0 = kpart + p.splits * (warp - 4); row0 < 128 && m0 + row0 < p.M && !dead;
+           row0 += p.splits * kWideConsumers * kRows) {
+        if constexpr (GATED) {
+          // lane l: outputs 4 l .. of the tile, whose gate columns lie at 128 (o / 64) + o % 64
+          // and the up columns 64 further: 256 bytes more for the upper 16 lanes
+          float4 g[kRows], u[kRows];
+          joined(g, row0, (lane >> 4) * 256);
+          joined(u, row0, (lane >> 4) * 256 + 256);
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) {
+            const int row = row0 + i * p.splits * kWideConsumers, m = m0 + row;
+            const float y[4] = {quant8::gate(g[i].x, p.gate_act) * u[i].x, quant8::gate(g[i].y, p.gate_act) * u[i].y,
+                                quant8::gate(g[i].z, p.gate_act) * u[i].z, quant8::gate(g[i].w, p.gate_act) * u[i].w};
+            float amax = quant8::max_nan(quant8::max_nan(fabsf(y[0]), fabsf(y[1]), fabsf(y[2])), fabsf(y[3]));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) amax = quant8::max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const float sc = quant8::scale_of(amax, quant8::kTopF8), inv = quant8::rcp(sc);
+            if (row >= 128 || m >= p.M) continue;
+            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.out) + int64_t(m) * p.out_st + nt * 128 + lane * 4) =
+                quant8::pack_e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+            if (lane == 0) p.q_scales[int64_t(m) * p.qs_st + nt] = sc;
+          }
+        } else {
+#pragma unroll 1
+          for (int h = 0; h < BN / 128; ++h) {
+            const int n = nt * BN + h * 128 + lane * 4;
+            float b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = n + e < p.N ? load_bias(p.bias, p.out_kind, n + e) : 0.f;
+            float4 v4[kRows];
+            joined(v4, row0, h * 512);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+              const int row = row0 + i * p.splits * kWideConsumers, m = m0 + row;
+              if (row >= 128 || m >= p.M) continue;
+              const float v[4] = {v4[i].x + b[0], v4[i].y + b[1], v4[i].z + b[2], v4[i].w + b[3]};
+              const int64_t at = int64_t(m) * p.out_st + n;
+              if (p.tma_out && n + 4 <= p.N) {   // rows on 16-byte boundaries: whole words
+                if (p.out_kind == kOutF32)
+                  *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+                else
+                  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+                      p.out_kind == kOutBf16 ? make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]))
+                                             : make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (n + e < p.N) store_one(p.out, p.out_kind, at + e, v[e]);
+              }
+            }
+          }
+        }
+      }
+    }
     if (lane == 0) tma::store_wait_read<0>();   // the staged rows have left shared memory
     if (dead) atomicExch(p.status, 1), s_abort = 1;
   }
@@ -669,7 +773,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
     // rank 0's barriers count the bytes of both CTAs and its thread issued all MMAs
     if (rank == 0 && tid == 0) drain_armed_loads(full_bar, S, armed);
     if (rank == 0 && warp == 1 && elect_one()) {
-      mma_commit_pair(&drain_bar);
+      mma_commit_pair(&drain_bar, lead);
       mbar_wait(&drain_bar, 0);
     }
   }
@@ -679,8 +783,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
 }
 
 template <int BN, bool GATED>
-int launch_wide(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
-                int dev, cudaStream_t st) {
+int launch_wide(Fp8GemmArgs p, int splits, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k,
+                int sms, int dev, cudaStream_t st) {
   using L = WideLayout<BN>;
   auto kernel = gemm_fp8_wide_kernel<BN, GATED>;
   static bool done[64] = {};
@@ -702,9 +806,55 @@ int launch_wide(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int64
                   tma::make_map_u8(&map_a, a, uint64_t(p.M), uint64_t(k), uint64_t(a_st), 128) &&
                   (!p.tma_out || tma::make_map_u8(&map_o, p.out, uint64_t(p.M), uint64_t(p.N) * bytes, uint64_t(o_st), 32)),
               "tensor map encoding failed");
-  const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
-  STRIX_CUDA(cluster::launch(kernel, unsigned(2 * pairs), 2u, kWideThreads, L::kSmem, st, p, map_w, map_a, map_o));
+#ifdef WSPL
+  splits = WSPL;
+#endif
+  p.splits = splits;
+  const int64_t pairs = splits > 1 || tiles < sms / 2 ? tiles * splits : sms / 2;
+  STRIX_CUDA(cluster::launch(kernel, unsigned(2 * pairs), unsigned(2 * splits), kWideThreads, L::kSmem, st, p, map_w, map_a, map_o));
   return launch_status("w8a8_fp8_gemm");
+}
+
+// Clusters of c pairs that the current device runs at once, c = 1 .. kMaxPairs (asked once;
+// all instantiations take an SM each).
+int pair_places(int dev, const int** out) {
+  static int places[64][kMaxPairs + 1] = {};
+  if (!places[dev][1]) {
+    auto kernel = gemm_fp8_wide_kernel<256, false>;
+    constexpr size_t smem = WideLayout<256>::kSmem;
+    STRIX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    for (int c = kMaxPairs; c >= 1; --c)
+      STRIX_CUDA(cluster::places(&places[dev][c], kernel, unsigned(2 * c), unsigned(kWideThreads), smem));
+    STRIX_CHECK(places[dev][1] > 0, "no room for a pair of CTAs");
+  }
+  *out = places[dev];
+  return STRIX_OK;
+}
+
+// Tile width and pairs per tile of the wide kernel, by the time each would take in ns. Fitted
+// to single rounds of 16 and 136 K blocks: a block costs a pair 372 on a tile of 256 x 256
+// and 272 on 256 x 128, a round of the larger tile 1,400 more at its ends; pairs that share a
+// tile need a place each at once, and their join costs 4,500 and 2,700. Measured at 128 x
+// 5,120 x 17,408: 256 wide 55.5 us with one pair per tile, 27.3 with three, 128 wide 40.5;
+// at 768 x 2,048 x 2,048: 11.0 and 8.3 us (one pair each); at 512 x 5,120 x 5,120: 20.9 and 24.8.
+struct WidePlan {
+  int bn, splits;
+};
+WidePlan wide_plan(int64_t m, int64_t n, int nkb, bool gated, const int* places) {
+  WidePlan best{256, 1};
+  int64_t least = INT64_MAX;
+  for (int bn : {256, 128}) {
+    if (gated && bn != 256) break;
+    const int64_t tiles = ((m + 255) / 256) * ((n + bn - 1) / bn);
+    const int64_t block = bn == 256 ? 372 : 272, ends = bn == 256 ? 1400 : 0, join = bn == 256 ? 4500 : 2700;
+    for (int c = 1; c <= kMaxPairs; ++c) {
+      if (c > 1 && (tiles > places[c] || nkb < 2 * c)) break;
+      const int64_t rounds = c > 1 ? 1 : (tiles + places[1] - 1) / places[1];
+      const int64_t t = rounds * ((nkb + c - 1) / c * block + ends) + (c > 1 ? join : 0);
+      if (t < least) least = t, best = {bn, c};
+    }
+  }
+  return best;
 }
 
 // The checks that both entry points share; fills what the kernels read of the operands.
@@ -742,12 +892,12 @@ int run_gemm(const Fp8GemmArgs& p, const void* a, int64_t a_st, const void* w, i
   if (p.M <= 16) return launch_stream<16, false>(p, a, a_st, w, w_st, k, sms, dev, st);
   if (p.M <= 32) return launch_stream<32, false>(p, a, a_st, w, w_st, k, sms, dev, st);
   if (p.M <= 64) return launch_stream<64, false>(p, a, a_st, w, w_st, k, sms, dev, st);
-  // Tiles of 256 x 128 while they all run at once: 0.72 of the time of one 256 x 256 tile
-  // (768 x 2,048 x 2,048: 8.1 against 11.0 us), but a second round costs more than the
-  // larger tile's one (512 x 5,120 x 5,120: 24.8 against 20.9 us).
-  const int64_t narrow = int64_t((p.M + 255) / 256) * ((p.N + 127) / 128);
-  if (narrow <= sms / 2) return launch_wide<128, false>(p, a, a_st, w, w_st, k, sms, dev, st);
-  return launch_wide<256, false>(p, a, a_st, w, w_st, k, sms, dev, st);
+  const int* places = nullptr;
+  const int rc = pair_places(dev, &places);
+  if (rc != STRIX_OK) return rc;
+  const WidePlan plan = wide_plan(p.M, p.N, p.nkb, false, places);
+  if (plan.bn == 128) return launch_wide<128, false>(p, plan.splits, a, a_st, w, w_st, k, sms, dev, st);
+  return launch_wide<256, false>(p, plan.splits, a, a_st, w, w_st, k, sms, dev, st);
 }
 
 }  // namespace
@@ -799,10 +949,16 @@ extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, con
   p.sa_sm = sa_stride_m, p.sa_sk = sa_stride_k, p.sw_sn = sw_stride_n, p.sw_sk = sw_stride_k;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (gated_in_one(n)) {
+    // (33 to 64 tokens: the weight stream took 40.0 and 44.9 us at 33 and 64 x 17,408 x 5,120, the
+    // wide tiles 42.9 and 43.3)
     p.out = q, p.out_st = q_stride, p.q_scales = scales, p.qs_st = s_stride, p.gate_act = gate_act;
     if (m <= 16) return launch_stream<16, true>(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
     if (m <= 32) return launch_stream<32, true>(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
-    return launch_wide<256, true>(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
+    const int* places = nullptr;
+    rc = pair_places(dev, &places);
+    if (rc != STRIX_OK) return rc;
+    const int splits = wide_plan(m, 2 * n, p.nkb, true, places).splits;
+    return launch_wide<256, true>(p, splits, a_q, a_stride, w, w_stride, k, sms, dev, st);
   }
   const int64_t need = m * 2 * n * 4;
   STRIX_CHECK(workspace_bytes >= need && workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,

@@ -308,8 +308,8 @@ __device__ __forceinline__ void mma_ss_lo(uint32_t tmem_d, uint32_t a_lo, uint32
 }
 
 // ----------------------------------------------------- pairs of CTAs (cta_group::2)
-// Two CTAs of a cluster share one MMA of M = 256: each holds its 128 rows of A, one
-// half of B's rows and the sums of its own rows. The CTA of rank 0 issues; tensor
+// Two CTAs of a cluster (ranks 2 i and 2 i + 1) share one MMA of M = 256: each holds its 128 rows
+// of A, one half of B's rows and the sums of its own rows. The even one issues; tensor
 // memory is taken and given back by both.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t cols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
@@ -333,13 +333,13 @@ __device__ __forceinline__ void mma_f8_pair(uint32_t tmem_d, uint32_t a_lo, uint
       : "memory");
 }
 
-// Arrives on the barrier at this offset in BOTH CTAs once every MMA issued so far by
-// this thread has completed.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// Arrives on the barrier at this offset in BOTH CTAs (of ranks `lead` and lead + 1 in the
+// cluster) once every MMA issued so far by this thread has completed.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint32_t lead) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_u32(bar)),
-      "h"(uint16_t(3))
+      "h"(uint16_t(3u << lead))
       : "memory");
 }
 

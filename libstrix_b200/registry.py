@@ -324,21 +324,25 @@ KERNELS: list[Kernel] = [
            "block. K % 16 == 0, any M and N, bias per channel",
            {"weight_bits": 8, "weight_dtype": "fp8_e4m3", "act_dtype": "fp8_e4m3", "group_size": 128,
             "dtype": ("bf16", "fp16", "fp32")},
-           {"tile": "128 weights x 16/32/64 tokens, up to 8 CTAs per tile along K joined through "
-                    "distributed shared memory",
-            "bound": "hbm"}),
+           {"tile": "128 weights x 16/32/64 tokens (rows <= 64), up to 8 CTAs per tile along K; 256 "
+                    "tokens x 256/128 weights per CTA pair, up to 4 pairs per tile along K",
+            "pipeline": "TMA ring, one issuing warp (cta_group::2 for the pairs), K blocks folded in "
+                        "fp32 by 4 / 8 warps, partial sums joined through distributed shared memory",
+            "bound": "hbm (rows <= 64) / tensor"}),
     Kernel("w8a8_fp8_gemm_act_mul_quant", "fp8_w8a8_gated",
            "the gate-up form of w8a8_fp8_gemm: act(gate) * up of the fp32 sums, out as e4m3 with "
            "one scale per (row, 128 columns)",
            {"weight_bits": 8, "weight_dtype": "fp8_e4m3", "act_dtype": "fp8_e4m3", "group_size": 128,
             "activation": ("silu", "gelu_tanh")},
-           {"bound": "hbm"}),
+           {"tile": "gate and up rows of 128 outputs; rows <= 32 weights as the MMA's M, beyond that "
+                    "256 tokens per CTA pair; other widths through an fp32 workspace",
+            "bound": "hbm (rows <= 32) / tensor"}),
     *[Kernel(f"rms_norm_quant_{form}", "rms_norm_quant",
              "root-mean-square norm with the residual's addition, out in 8 bits with scales; a row "
              "is read once and stays in registers",
              {"dtype": ("bf16", "fp16"), "activation_dtype": q, "group_size": group,
               "residual": (True, False)},
-             {"unit": "one CTA per row", "bound": "hbm"})
+             {"unit": "persistent CTAs, one row at a time", "bound": "hbm"})
       for form, q, group in (("fp8", "fp8_e4m3", 128), ("token_i8", "int8", 0))],
     *[Kernel(f"act_mul_quant_{form}", "act_mul_quant",
              "act(gate) * up of gate-up rows, out in 8 bits with scales",

@@ -292,7 +292,8 @@ def test_gemm_ragged(m, n, k, out_dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(1, 34816, 5120), (16, 5120, 17408), (700, 2560, 5120), (1500, 1024, 2048)])
+@pytest.mark.parametrize("m,n,k", [(1, 34816, 5120), (16, 5120, 17408), (700, 2560, 5120), (1500, 1024, 2048),
+                                   (128, 5120, 17408), (100, 1000, 8192), (65, 513, 16384), (250, 4000, 5120)])
 def test_gemm_at_layer_widths(m, n, k):
     check_gemm(m, n, k, seed=2)
 
@@ -414,7 +415,9 @@ def test_empty_batches():
 @pytest.mark.gpu
 @pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
 @pytest.mark.parametrize("m,n,k", [(1, 16, 128), (2, 768, 2048), (16, 144, 272), (33, 512, 384), (65, 400, 1040),
-                                   (256, 768, 2048), (300, 640, 528), (1000, 1024, 2048), (515, 2880, 1152)])
+                                   (256, 768, 2048), (300, 640, 528), (1000, 1024, 2048), (515, 2880, 1152),
+                                   (17, 1152, 528), (40, 256, 1040), (64, 768, 2048), (70, 256, 4112), (300, 384, 6016),
+                                   (257, 128, 9000 // 16 * 16)])
 def test_gated_product(m, n, k, activation):
     a, sa, w, sw = gemm_case(m, 2 * n, k, 6)
     sa = sa * 0.03                                       # gates of a few units
