@@ -180,7 +180,7 @@ struct ActArgs {
   uint8_t* q;
   float* scales;
   int64_t x_st, q_st, s_st, rows;
-  int k8, act;
+  int k8;
 };
 
 // IN: 0 bf16, 1 fp16, 2 fp32
@@ -197,7 +197,7 @@ __device__ __forceinline__ void load8(const void* base, int64_t elem, float (&v)
 
 // y[u] = act(gate) * up of vector c[u] of row[u], for the U vectors with c[u] < k8; all
 // loads are issued before the first is used.
-template <int IN, int U>
+template <int IN, bool GELU, int U>
 __device__ __forceinline__ void gated8(const ActArgs& p, const int64_t (&row)[U], const int (&c)[U],
                                        float (&y)[U][8]) {
   if constexpr (IN == 2) {
@@ -208,7 +208,7 @@ __device__ __forceinline__ void gated8(const ActArgs& p, const int64_t (&row)[U]
       load8<IN>(p.x, row[u] * p.x_st + c[u] * 8, y[u]);
       load8<IN>(p.x, row[u] * p.x_st + (p.k8 + c[u]) * 8, up);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[u][j] = gate(y[u][j], p.act) * up[j];
+      for (int j = 0; j < 8; ++j) y[u][j] = gate<GELU>(y[u][j]) * up[j];
     }
   } else {
     uint4 g[U], h[U];
@@ -224,14 +224,14 @@ __device__ __forceinline__ void gated8(const ActArgs& p, const int64_t (&row)[U]
       float up[8];
       unpack8<IN == 1>(g[u], y[u]), unpack8<IN == 1>(h[u], up);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[u][j] = gate(y[u][j], p.act) * up[j];
+      for (int j = 0; j < 8; ++j) y[u][j] = gate<GELU>(y[u][j]) * up[j];
     }
   }
 }
 
 // e4m3, a scale per 128 columns: a team of 16 lanes per (row, group), no exchange
 // beyond the team. A team takes U groups, their loads first.
-template <int IN, int U>
+template <int IN, bool GELU, int U>
 __global__ void __launch_bounds__(256) act_mul_quant_fp8_kernel(const ActArgs p) {
   pdl_enter();
   const int groups = (p.k8 + 15) >> 4, sub = threadIdx.x & 15;
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256) act_mul_quant_fp8_kernel(const ActArgs p)
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[u][j] = 0.f;
   }
-  gated8<IN, U>(p, row, c, y);
+  gated8<IN, GELU, U>(p, row, c, y);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const float s = scale_of(group_max(abs_max8(y[u])), kTopF8);
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(256) act_mul_quant_fp8_kernel(const ActArgs p)
 }
 
 // int8, a scale per row: one CTA per row, the row in registers as in the norm.
-template <int IN, int V>
+template <int IN, bool GELU, int V>
 __global__ void __launch_bounds__(kMaxRowThreads) act_mul_quant_token_kernel(const ActArgs p) {
   pdl_enter();
   __shared__ float s_max[32];
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kMaxRowThreads) act_mul_quant_token_kernel(con
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[i][j] = 0.f;
   }
-  gated8<IN, V>(p, rows, c, y);
+  gated8<IN, GELU, V>(p, rows, c, y);
   float m = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) m = max_nan(m, abs_max8(y[i]));
@@ -346,22 +346,29 @@ int launch_norm(const NormArgs& p, cudaStream_t st) {
   return launch_norm_v<F8, F16, WF32, 8>(p, s.threads, sms, dev, st);
 }
 
-template <int IN>
+template <int IN, bool GELU>
 int launch_act(const ActArgs& p, bool fp8, cudaStream_t st) {
   if (fp8) {
     const int64_t teams = p.rows * ((p.k8 + 15) / 16);
     // two groups per team once there are more than four CTAs of one per SM
-    if (teams > 16 * 4 * 148) launch_chain(act_mul_quant_fp8_kernel<IN, 2>, unsigned((teams + 31) / 32), 256, 0, st, p);
-    else launch_chain(act_mul_quant_fp8_kernel<IN, 1>, unsigned((teams + 15) / 16), 256, 0, st, p);
+    if (teams > 16 * 4 * 148)
+      launch_chain(act_mul_quant_fp8_kernel<IN, GELU, 2>, unsigned((teams + 31) / 32), 256, 0, st, p);
+    else
+      launch_chain(act_mul_quant_fp8_kernel<IN, GELU, 1>, unsigned((teams + 15) / 16), 256, 0, st, p);
   } else {
     const RowShape s = row_shape(p.k8, 1);
     const unsigned grid = unsigned(p.rows);
-    if (s.v == 1) launch_chain(act_mul_quant_token_kernel<IN, 1>, grid, s.threads, 0, st, p);
-    else if (s.v == 2) launch_chain(act_mul_quant_token_kernel<IN, 2>, grid, s.threads, 0, st, p);
-    else if (s.v == 4) launch_chain(act_mul_quant_token_kernel<IN, 4>, grid, s.threads, 0, st, p);
-    else launch_chain(act_mul_quant_token_kernel<IN, 8>, grid, s.threads, 0, st, p);
+    if (s.v == 1) launch_chain(act_mul_quant_token_kernel<IN, GELU, 1>, grid, s.threads, 0, st, p);
+    else if (s.v == 2) launch_chain(act_mul_quant_token_kernel<IN, GELU, 2>, grid, s.threads, 0, st, p);
+    else if (s.v == 4) launch_chain(act_mul_quant_token_kernel<IN, GELU, 4>, grid, s.threads, 0, st, p);
+    else launch_chain(act_mul_quant_token_kernel<IN, GELU, 8>, grid, s.threads, 0, st, p);
   }
   return launch_status("act_mul_quant");
+}
+
+template <int IN>
+int launch_act(const ActArgs& p, int act, bool fp8, cudaStream_t st) {
+  return act == 1 ? launch_act<IN, false>(p, fp8, st) : launch_act<IN, true>(p, fp8, st);
 }
 
 }  // namespace
@@ -434,9 +441,9 @@ extern "C" int strix_act_mul_quant(const void* x, void* q, float* scales, int64_
   ActArgs p;
   p.x = x, p.q = static_cast<uint8_t*>(q), p.scales = scales;
   p.x_st = x_stride, p.q_st = q_stride, p.s_st = s_stride, p.rows = rows;
-  p.k8 = int(k / 8), p.act = gate_act;
+  p.k8 = int(k / 8);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (in_type == 0) return launch_act<0>(p, fp8 != 0, st);
-  if (in_type == 1) return launch_act<1>(p, fp8 != 0, st);
-  return launch_act<2>(p, fp8 != 0, st);
+  if (in_type == 0) return launch_act<0>(p, gate_act, fp8 != 0, st);
+  if (in_type == 1) return launch_act<1>(p, gate_act, fp8 != 0, st);
+  return launch_act<2>(p, gate_act, fp8 != 0, st);
 }

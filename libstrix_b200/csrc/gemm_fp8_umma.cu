@@ -376,6 +376,9 @@ __device__ __forceinline__ void fold2(float& a0, float& a1, uint32_t r0, uint32_
       : "r"(r0), "r"(r1), "l"(f2));
 }
 
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x16(taddr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32(taddr, r); }
+
 constexpr int kMaxPairs = 4;   // pairs of CTAs that share a tile along K
 
 template <int BN>
@@ -497,9 +500,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
     }
     if (p.splits > 1) cluster::sync();   // the folding warps' exchange of partial sums
   } else {
-    // 128 x 40 + 256 x this stays within the launch's 384 x 168; of the values that do, the
-    // ones at which the compiler spills nothing in the loop
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(GATED ? 176 : 232));
+    // 128 x 40 + 256 x 232 registers: the launch's 384 x 168
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int trow = (warp & 3) * 32 + lane;          // TMEM lane = token of this CTA's 128
     const int cg = (warp - 4) >> 2;                   // which half of the BN columns
     const uint32_t src0 = tmem + (uint32_t((warp & 3) * 32) << 16) + cg * NC;
@@ -536,14 +538,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
         }
         tc_fence_after_sync();
         const uint32_t src = src0 + b * BN;
-        constexpr int CH = 32;
+        // columns per load, two loads in registers: the gated form's second scale leaves room
+        // for 16 only (with 32 the loop spills at most register budgets)
+        constexpr int CH = GATED ? 16 : 32;
         uint32_t r[2][CH];
-        tmem_ld_32x32(src, r[0]);
+        tmem_ld(src, r[0]);
 #pragma unroll
         for (int c = 0; c < NC / CH; ++c) {
           tmem_ld_wait();
           if (c + 1 < NC / CH) {
-            tmem_ld_32x32(src + (c + 1) * CH, r[(c + 1) & 1]);
+            tmem_ld(src + (c + 1) * CH, r[(c + 1) & 1]);
           } else {   // everything read: the accumulator may be written again
             tc_fence_before_sync();
             __syncwarp();
@@ -551,7 +555,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
           }
 #pragma unroll
           for (int j = 0; j < CH; j += 2) {
-            fold2(acc[c * CH + j], acc[c * CH + j + 1], r[c & 1][j], r[c & 1][j + 1], GATED && c >= 2 ? fu2 : f2);
+            fold2(acc[c * CH + j], acc[c * CH + j + 1], r[c & 1][j], r[c & 1][j + 1], GATED && c * CH >= 64 ? fu2 : f2);
           }
         }
         if (++s == S) s = 0, ph ^= 1;
