@@ -23,8 +23,8 @@ def _eager(x) -> bool:
     a call's 26, more than the smallest kernels run): an ordinary CUDA tensor outside a
     trace. Anything else (fake tensors, subclasses, CPU tensors, a dispatch mode such as a
     tracer's, torch.compile) takes torch.ops.strix, with its shape inference and errors."""
-    return (type(x) is torch.Tensor and x.is_cuda and torch._C._len_torch_dispatch_stack() == 0
-            and not torch._C._is_tracing() and not torch.compiler.is_compiling())
+    return (not torch.compiler.is_compiling() and type(x) is torch.Tensor and x.is_cuda
+            and torch._C._len_torch_dispatch_stack() == 0 and not torch._C._is_tracing())
 
 
 def _is_fp8(q_dtype: torch.dtype) -> bool:

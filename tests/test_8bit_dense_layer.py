@@ -600,6 +600,17 @@ def test_a_tracer_sees_the_ops():
 
 
 @pytest.mark.gpu
+def test_a_compiled_caller_keeps_one_graph():
+    x, r, w = norm_case(5, 256, torch.bfloat16, 41)
+    _, _, w13, s13 = gemm_case(1, 512, 256, 42)
+    _, _, w2, s2 = gemm_case(1, 256, 256, 43)
+    args = [t.to(DEV) for t in (x, w, w13, s13, w2, s2)]
+    rd = r.to(DEV)
+    compiled = torch.compile(lambda *a: dense.fused_mlp_fp8_w8a8(*a, residual=rd), backend="eager", fullgraph=True)
+    assert torch.equal(compiled(*args), dense.fused_mlp_fp8_w8a8(*args, residual=rd))
+
+
+@pytest.mark.gpu
 def test_ops_check_their_tensors():
     ops = torch.ops.strix
     a, sa, w, sw = (t.to(DEV) for t in gemm_case(4, 256, 256))
