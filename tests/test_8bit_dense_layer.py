@@ -554,6 +554,69 @@ def test_vllm_linear_with_8_bit_activations(m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_dtype", [F8, torch.int8])
+def test_norm_and_act_beyond_32_bit_offsets(q_dtype):
+    """2.2 billion elements in, the last rows against the oracle."""
+    m, k = 33100, 65536
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(DEV).manual_seed(50)
+    at = torch.tensor([0, 5, 16384, 32767, 32768, m - 2, m - 1])
+    x[at.to(DEV)] = torch.randn(len(at), k, generator=g, device=DEV).bfloat16()
+    w = (1 + 0.1 * torch.randn(k, generator=gen(51))).bfloat16()
+    q, s = dense.rms_norm_quant(x, w.to(DEV), 1e-6, x, x, q_dtype=q_dtype)     # in place: 2 x
+    rows = x[at.to(DEV)].cpu()
+    check_rows(q[at.to(DEV)], s[at.to(DEV)], O.rms_norm(rows, w, 1e-6)[1], q_dtype == F8, Y_REL)
+    assert not q[1].float().any() and not q[m - 3].float().any()
+    q, s = dense.act_mul_quant(x, q_dtype=q_dtype)
+    check_rows(q[at.to(DEV)], s[at.to(DEV)], O.act_mul(rows, "silu"), q_dtype == F8, GATE_REL)
+
+
+@pytest.mark.gpu
+def test_products_beyond_32_bit_offsets():
+    """An output of 2.3 billion elements (and a gated one), rows and columns at its ends."""
+    n, k = 33000, 144
+    m = 70000
+    a, sa, w, sw = gemm_case(64, n, k, 52)
+    big_a = torch.zeros(m, k, device=DEV).to(F8)
+    big_sa = torch.ones(m, 2, device=DEV)
+    at = torch.cat([torch.arange(0, 32), torch.arange(m - 32, m)])
+    big_a.view(torch.uint8)[at.to(DEV)] = a.view(torch.uint8).to(DEV)
+    big_sa[at.to(DEV)] = sa.to(DEV)
+    out = dense.fp8_gemm(big_a, big_sa, w.to(DEV), sw.to(DEV))
+    status_ok()
+    ref, err = O.fp8_gemm(a, sa, w, sw), gemm_error(a, sa, w, sw)
+    got = out[at.to(DEV)].double().cpu()
+    assert ((got - ref).abs() <= err + 2.0 ** -8 * (ref.abs() + err)).all()
+    assert not out[32:m - 32:997].any()
+    del out
+    w2, sw2 = w[:2048].contiguous(), sw[:16].contiguous()
+    q, s = dense.fp8_gemm_act_mul_quant(big_a, big_sa, w2.to(DEV), sw2.to(DEV))
+    q1, s1 = dense.fp8_gemm_act_mul_quant(a.to(DEV), sa.to(DEV), w2.to(DEV), sw2.to(DEV))
+    status_ok()
+    assert torch.allclose(s[at.to(DEV)], s1, rtol=1e-5, atol=0) and (s[32] == 1).all()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls that overlap on the GPU share nothing."""
+    cases = [gemm_case(m, n, k, 60) for m, n, k in ((3, 1024, 4096), (200, 1024, 2048), (50, 512, 4096), (90, 256, 8192))]
+    cases = [[t.to(DEV) for t in c] for c in cases]
+    want = [(dense.fp8_gemm(*c), dense.fp8_gemm_act_mul_quant(*c)) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 4]):
+            c = cases[i % 4 if i < 8 else 3 - i % 4]
+            got.append((dense.fp8_gemm(*c), dense.fp8_gemm_act_mul_quant(*c)))
+    torch.cuda.synchronize()
+    status_ok()
+    for i, (o, (q, s)) in enumerate(got):
+        w_o, (w_q, w_s) = want[i % 4 if i < 8 else 3 - i % 4]
+        assert torch.equal(o, w_o) and torch.equal(q.view(torch.uint8), w_q.view(torch.uint8)) and torch.equal(s, w_s)
+
+
+@pytest.mark.gpu
 def test_results_do_not_change_from_run_to_run():
     for m, n, k in ((1, 512, 4096), (50, 1024, 2048), (600, 2048, 1024)):
         a, sa, w, sw = (t.to(DEV) for t in gemm_case(m, n, k, 9))
