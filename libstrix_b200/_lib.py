@@ -67,6 +67,7 @@ class StrixError(RuntimeError):
 
 _lib = None
 _protos: dict[str, tuple] = {}
+_functions: dict = {}      # name -> typed entry point, filled by call()
 
 
 def load() -> ctypes.CDLL:
@@ -101,10 +102,12 @@ def prototypes() -> dict[str, tuple]:
 
 def call(name: str, *args) -> None:
     """Calls a status-returning entry point; raises StrixError with the library's message."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
+    rc = fn(*args)
     if rc != STRIX_OK:
-        msg = lib.strix_last_error().decode("utf-8", "replace")
+        msg = load().strix_last_error().decode("utf-8", "replace")
         raise StrixError(msg or f"{name} failed with status {rc}")
 
 

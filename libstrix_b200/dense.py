@@ -12,6 +12,8 @@ python/strix_vllm/fp8.py:121-262), with vLLM's 16-bit norm and silu_and_mul betw
 from __future__ import annotations
 
 import torch
+from torch._C import _is_tracing, _len_torch_dispatch_stack
+from torch.compiler import is_compiling
 
 from . import torch_ops
 
@@ -23,8 +25,8 @@ def _eager(x) -> bool:
     a call's 26, more than the smallest kernels run): an ordinary CUDA tensor outside a
     trace. Anything else (fake tensors, subclasses, CPU tensors, a dispatch mode such as a
     tracer's, torch.compile) takes torch.ops.strix, with its shape inference and errors."""
-    return (not torch.compiler.is_compiling() and type(x) is torch.Tensor and x.is_cuda
-            and torch._C._len_torch_dispatch_stack() == 0 and not torch._C._is_tracing())
+    return (not is_compiling() and type(x) is torch.Tensor and x.is_cuda
+            and _len_torch_dispatch_stack() == 0 and not _is_tracing())
 
 
 def _is_fp8(q_dtype: torch.dtype) -> bool:
@@ -41,17 +43,21 @@ def rms_norm_quant(x, weight, eps: float = 1e-6, residual=None, residual_out=Non
     itself for an update in place. The norm is taken of the fp32 sum, before that
     rounding. q_dtype float8_e4m3fn: scales fp32 [M, ceil(K / 128)], K a multiple of 16;
     int8: scales fp32 [M], K a multiple of 8."""
-    ns = torch_ops if _eager(x) else torch.ops.strix
-    op = ns.rms_norm_quant_fp8 if _is_fp8(q_dtype) else ns.rms_norm_quant_token_i8
-    return op(x, weight, eps, residual, residual_out)
+    fp8 = _is_fp8(q_dtype)
+    if _eager(x):
+        return torch_ops._rms_norm_quant(x, weight, eps, residual, residual_out, fp8)
+    ops = torch.ops.strix
+    return (ops.rms_norm_quant_fp8 if fp8 else ops.rms_norm_quant_token_i8)(x, weight, eps, residual, residual_out)
 
 
 def act_mul_quant(x, activation: str = "silu", q_dtype=FP8):
     """(q, scales) of act(x[:, :K]) * x[:, K:] for x [M, 2 K] (bf16, fp16 or fp32),
     activation silu or gelu_tanh; q and scales as rms_norm_quant returns them."""
-    ns = torch_ops if _eager(x) else torch.ops.strix
-    op = ns.act_mul_quant_fp8 if _is_fp8(q_dtype) else ns.act_mul_quant_token_i8
-    return op(x, activation)
+    fp8 = _is_fp8(q_dtype)
+    if _eager(x):
+        return torch_ops._act_mul_quant(x, activation, fp8)
+    ops = torch.ops.strix
+    return (ops.act_mul_quant_fp8 if fp8 else ops.act_mul_quant_token_i8)(x, activation)
 
 
 def fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
