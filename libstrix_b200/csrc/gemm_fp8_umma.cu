@@ -55,6 +55,9 @@ __device__ __forceinline__ void store_one(void* out, int kind, int64_t at, float
   else static_cast<float*>(out)[at] = v;
 }
 
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x16(taddr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32(taddr, r); }
+
 // ================================================================ weight stream
 // Few tokens: the weights are the MMA's A operand (128 rows fill M whatever the
 // batch), NB tokens its N, and the kernel is a stream of the weights. A cluster of
@@ -121,10 +124,9 @@ __global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayou
   tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0), ring_s = smem_u32(ring);
 
-  constexpr int NC = NB;
-  float acc[NC];
+  float acc[NB];
 #pragma unroll
-  for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+  for (int j = 0; j < NB; ++j) acc[j] = 0.f;
 
   if (warp == 0) {
     const bool one = elect_one();
@@ -213,18 +215,26 @@ __global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayou
       }
       tc_fence_after_sync();
       const float4* sc = reinterpret_cast<const float4*>(s_scale + s * NB);
+      // loads of tensor memory CH columns at a time, the next one under way behind the sums;
+      // two products per instruction: scale * weight scale, and its multiply-add
+      constexpr int CH = NB < 32 ? NB : 32;
+      const uint32_t src = tmem + lane_base + (b * T + part_of) * NB;
+      const float2 w2 = make_float2(ws, ws);
+      uint32_t r[2][CH];
+      tmem_ld(src, r[0]);
 #pragma unroll
-      for (int c = 0; c < NC; c += 16) {
-        uint32_t r[16];
-        tmem_ld_32x16(tmem + lane_base + (b * T + part_of) * NB + c, r);
+      for (int c = 0; c < NB / CH; ++c) {
         tmem_ld_wait();
+        if (c + 1 < NB / CH) tmem_ld(src + (c + 1) * CH, r[(c + 1) & 1]);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 q = sc[(c + j) >> 2];
-          acc[c + j] += __uint_as_float(r[j]) * (q.x * ws);
-          acc[c + j + 1] += __uint_as_float(r[j + 1]) * (q.y * ws);
-          acc[c + j + 2] += __uint_as_float(r[j + 2]) * (q.z * ws);
-          acc[c + j + 3] += __uint_as_float(r[j + 3]) * (q.w * ws);
+        for (int j = 0; j < CH; j += 4) {
+          const float4 q = sc[(c * CH + j) >> 2];
+          const float2 f0 = __fmul2_rn(make_float2(q.x, q.y), w2), f1 = __fmul2_rn(make_float2(q.z, q.w), w2);
+          const uint32_t* x = &r[c & 1][j];
+          float* a = &acc[c * CH + j];
+          const float2 s0 = __ffma2_rn(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), f0, make_float2(a[0], a[1]));
+          const float2 s1 = __ffma2_rn(make_float2(__uint_as_float(x[2]), __uint_as_float(x[3])), f1, make_float2(a[2], a[3]));
+          a[0] = s0.x, a[1] = s0.y, a[2] = s1.x, a[3] = s1.y;
         }
       }
       tc_fence_before_sync();
@@ -375,9 +385,6 @@ __device__ __forceinline__ void fold2(float& a0, float& a1, uint32_t r0, uint32_
       : "+f"(a0), "+f"(a1)
       : "r"(r0), "r"(r1), "l"(f2));
 }
-
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x16(taddr, r); }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32(taddr, r); }
 
 constexpr int kMaxPairs = 4;   // pairs of CTAs that share a tile along K
 
