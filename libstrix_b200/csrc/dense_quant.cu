@@ -74,6 +74,10 @@ struct NormArgs {
 // fp32 registers, and stay in flight through its reductions; the weights stay in
 // registers (as 16-bit pairs) for all rows. The sum may replace x or the residual in
 // place: no row is read by two CTAs, and a row is read before any of it is written.
+// Measured (bf16, residual): 4,096 x 5,120 23.5 us, 8,192 x 5,120 47 us = 6.2 TB/s (a CTA per row
+// without the row ahead: 34 and 63 us); one row of 5,120 2.3 us, a launch and its latency.
+// Two vectors per thread need 64 registers; four (rows beyond 16,384 columns) have none left
+// for the row ahead: 2,000 x 32,768 82 us = 5.6 TB/s.
 template <bool F8, bool F16, bool WF32, int V>
 __global__ void __launch_bounds__(kMaxRowThreads) rms_norm_quant_kernel(const NormArgs p) {
   pdl_enter();
@@ -230,7 +234,9 @@ __device__ __forceinline__ void gated8(const ActArgs& p, const int64_t (&row)[U]
 }
 
 // e4m3, a scale per 128 columns: a team of 16 lanes per (row, group), no exchange
-// beyond the team. A team takes U groups, their loads first.
+// beyond the team. A team takes U groups, their loads first. Measured: 4,096 x 17,408
+// bf16 60 us = 6.0 TB/s, at four fifths of the issue slots (27 instructions per output, of
+// which an exponential, a reciprocal and half a conversion go to the slow units).
 template <int IN, bool GELU, int U>
 __global__ void __launch_bounds__(256) act_mul_quant_fp8_kernel(const ActArgs p) {
   pdl_enter();
@@ -260,7 +266,8 @@ __global__ void __launch_bounds__(256) act_mul_quant_fp8_kernel(const ActArgs p)
   }
 }
 
-// int8, a scale per row: one CTA per row, the row in registers as in the norm.
+// int8, a scale per row: one CTA per row, the row in registers as in the norm. Measured:
+// 8,192 x 2,560 bf16 18 us = 5.8 TB/s; 16 x 17,408 5.5 us (16 CTAs, their latency).
 template <int IN, bool GELU, int V>
 __global__ void __launch_bounds__(kMaxRowThreads) act_mul_quant_token_kernel(const ActArgs p) {
   pdl_enter();
