@@ -14,7 +14,6 @@
 // Bound: HBM. Bytes per element: norm 2 + 2 read, 2 + 1 written (residual form);
 // act 4 read, 1 written. A row stays in registers between its statistics and its
 // rounding, so it is read once.
-#include "cluster.cuh"
 #include "quant8.cuh"
 
 namespace strix {
@@ -356,9 +355,12 @@ int launch_norm(const NormArgs& p, cudaStream_t st) {
 template <int IN, bool GELU>
 int launch_act(const ActArgs& p, bool fp8, cudaStream_t st) {
   if (fp8) {
+    int dev = 0, sms = 0;
+    const int rc = device_sms(dev, sms);
+    if (rc != STRIX_OK) return rc;
     const int64_t teams = p.rows * ((p.k8 + 15) / 16);
-    // two groups per team once there are more than four CTAs of one per SM
-    if (teams > 16 * 4 * 148)
+    // two groups per team once that still leaves two CTAs per SM
+    if (teams > int64_t(sms) * 64)
       launch_chain(act_mul_quant_fp8_kernel<IN, GELU, 2>, unsigned((teams + 31) / 32), 256, 0, st, p);
     else
       launch_chain(act_mul_quant_fp8_kernel<IN, GELU, 1>, unsigned((teams + 15) / 16), 256, 0, st, p);
