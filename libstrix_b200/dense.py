@@ -12,21 +12,53 @@ python/strix_vllm/fp8.py:121-262), with vLLM's 16-bit norm and silu_and_mul betw
 from __future__ import annotations
 
 import torch
-from torch._C import _is_tracing, _len_torch_dispatch_stack
+from torch.autograd import forward_ad
 from torch.compiler import is_compiling
 
 from . import torch_ops
 
+try:   # not part of torch's public interface: without them every call takes the dispatcher
+    from torch._C import _are_functorch_transforms_active, _is_tracing, _len_torch_dispatch_stack
+except ImportError:
+    _are_functorch_transforms_active = None
+
 FP8 = torch.float8_e4m3fn
 
 
-def _eager(x) -> bool:
+def _plain(*tensors) -> bool:
+    """Whether a call on these operands (None: absent) is an ordinary one: no tracer's or
+    other dispatch mode, no torch.func transform, no subclass among them (fake tensors,
+    wrappers) and no derivative asked for. The operators have none: with requires_grad the
+    dispatcher attaches a node that warns in the backward pass, and a forward-mode tangent
+    would be lost without a word there too, so it is refused here."""
+    if (_are_functorch_transforms_active is None or _are_functorch_transforms_active()
+            or _len_torch_dispatch_stack() != 0 or _is_tracing()):
+        return False
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is None:
+            continue
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter or grad and t.requires_grad:
+            return False
+    return True
+
+
+def _no_tangents(*tensors) -> None:
+    if getattr(forward_ad, "_current_level", 0) >= 0:   # a dual level is open
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the 8-bit dense layer has no forward-mode derivative")
+
+
+def _eager(first, *others) -> bool:
     """Whether a call may go to the op's implementation without the dispatcher (4 us of
-    a call's 26, more than the smallest kernels run): an ordinary CUDA tensor outside a
-    trace. Anything else (fake tensors, subclasses, CPU tensors, a dispatch mode such as a
-    tracer's, torch.compile) takes torch.ops.strix, with its shape inference and errors."""
-    return (not is_compiling() and type(x) is torch.Tensor and x.is_cuda
-            and _len_torch_dispatch_stack() == 0 and not _is_tracing())
+    a call's 26, more than the smallest kernels run): plain CUDA tensors only, and CUDA
+    as the first operand says (the implementation checks that the others are with it).
+    Anything else takes torch.ops.strix, with its shape inference and errors."""
+    if is_compiling():
+        return False
+    _no_tangents(first, *others)
+    return first.is_cuda and _plain(first, *others)
 
 
 def _is_fp8(q_dtype: torch.dtype) -> bool:
@@ -44,7 +76,7 @@ def rms_norm_quant(x, weight, eps: float = 1e-6, residual=None, residual_out=Non
     rounding. q_dtype float8_e4m3fn: scales fp32 [M, ceil(K / 128)], K a multiple of 16;
     int8: scales fp32 [M], K a multiple of 8."""
     fp8 = _is_fp8(q_dtype)
-    if _eager(x):
+    if _eager(x, weight, residual, residual_out):
         return torch_ops._rms_norm_quant(x, weight, eps, residual, residual_out, fp8)
     ops = torch.ops.strix
     return (ops.rms_norm_quant_fp8 if fp8 else ops.rms_norm_quant_token_i8)(x, weight, eps, residual, residual_out)
@@ -63,7 +95,7 @@ def act_mul_quant(x, activation: str = "silu", q_dtype=FP8):
 def fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
     """[M, N] of a_q e4m3 [M, K] (a_scale fp32 [M, ceil(K / 128)]) and w e4m3 [N, K]
     (w_scale fp32 [ceil(N / 128), ceil(K / 128)]), K a multiple of 16."""
-    ns = torch_ops if _eager(a_q) else torch.ops.strix
+    ns = torch_ops if _eager(a_q, a_scale, w, w_scale, bias) else torch.ops.strix
     return ns.w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias, out_dtype)
 
 
@@ -71,7 +103,7 @@ def fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation: str = "silu"):
     """(q e4m3 [M, N], scales) of act(gate) * up, where w e4m3 [2 N, K] holds the gate
     rows and then the up rows: fp8_gemm and act_mul_quant without the 16-bit rows
     between them."""
-    ns = torch_ops if _eager(a_q) else torch.ops.strix
+    ns = torch_ops if _eager(a_q, a_scale, w, w_scale) else torch.ops.strix
     return ns.w8a8_fp8_gemm_act_mul_quant(a_q, a_scale, w, w_scale, activation)
 
 

@@ -1,0 +1,100 @@
+"""The 8-bit dense layer at the calls between its main ones: transforms and derivatives,
+a single row of any stride, non-finite and empty groups through each join of the gated
+product, strided operands there, overlapping streams, offsets beyond 32 bits. Bounds as
+in test_8bit_dense_layer.py."""
+
+import warnings
+
+import pytest
+import torch
+
+from libstrix_b200 import dense
+from test_8bit_dense_layer import DEV, gemm_case, norm_case
+
+
+# ------------------------------------------------- transforms and derivatives
+def calls(device):
+    """Each public call on small operands, with the operand that may be wrapped first."""
+    x, r, w = (t.to(device) for t in norm_case(4, 256, torch.bfloat16, 1))
+    a, sa, wq, sw = (t.to(device) for t in gemm_case(4, 256, 256))
+    bias = torch.ones(256, device=device).bfloat16()
+    return {
+        "norm": (lambda t: dense.rms_norm_quant(t, w, residual=r)[1], x),
+        "norm_weight": (lambda t: dense.rms_norm_quant(x, t)[1], w),
+        "norm_residual": (lambda t: dense.rms_norm_quant(x, w, residual=t)[1], r),
+        "act": (lambda t: dense.act_mul_quant(t)[1], x),
+        "gemm_scale": (lambda t: dense.fp8_gemm(a, t, wq, sw), sa),
+        "gemm_weight_scale": (lambda t: dense.fp8_gemm(a, sa, wq, t), sw),
+        "gemm_bias": (lambda t: dense.fp8_gemm(a, sa, wq, sw, t), bias),
+        "gated_scale": (lambda t: dense.fp8_gemm_act_mul_quant(a, t, wq, sw)[1], sa),
+    }
+
+
+class Wrapped(torch.Tensor):
+    pass
+
+
+def test_only_ordinary_calls_skip_the_dispatcher():
+    x, w = torch.randn(3, 4), torch.randn(4)
+    assert dense._plain(x, w, None)
+    assert dense._plain(x, torch.nn.Parameter(w, requires_grad=False))
+    assert not dense._plain(x, w.as_subclass(Wrapped)) and not dense._plain(x.as_subclass(Wrapped), w)
+    p = torch.nn.Parameter(w)
+    assert not dense._plain(x, p)
+    with torch.no_grad():
+        assert dense._plain(x, p)
+    seen = []
+
+    def look(t):
+        seen.append(dense._plain(t, w))
+        return (t * 2).sum()
+
+    torch.func.vmap(look)(x)
+    torch.func.grad(look)(w)
+    torch.func.vmap(lambda t: look(x) + t.sum())(x)      # an operand from outside the transform
+    assert seen == [False, False, False]
+
+
+def test_direct_path_needs_no_private_names(monkeypatch):
+    monkeypatch.setattr(dense, "_are_functorch_transforms_active", None)
+    assert not dense._plain(torch.randn(3))
+
+
+@pytest.mark.parametrize("name", calls("cpu"))
+def test_forward_mode_is_refused(name):
+    from torch.autograd import forward_ad
+
+    f, t = calls("cpu")[name]
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            f(forward_ad.make_dual(t, torch.ones_like(t)))
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(f, (t,), (torch.ones_like(t),))
+
+
+@pytest.mark.gpu
+def test_vmap_runs_the_products_and_names_what_it_cannot():
+    x = norm_case(6, 256, torch.bfloat16, 1, False)[0].to(DEV).view(2, 3, 256)
+    a, sa, w, sw = (t.to(DEV) for t in gemm_case(6, 256, 256))
+    a3, sa3 = a.view(2, 3, 256), sa.view(2, 3, 2)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")                  # "performance drop": torch's fallback loops
+        out = torch.func.vmap(lambda s: dense.fp8_gemm(a3[0], s, w, sw))(sa3)
+        s = torch.func.vmap(lambda t: dense.act_mul_quant(t)[1])(x)
+    for i in range(2):
+        assert torch.equal(out[i], dense.fp8_gemm(a3[0], sa3[i], w, sw))
+        assert torch.equal(s[i], dense.act_mul_quant(x[i])[1])
+    with pytest.raises(RuntimeError, match="[Bb]atching rule"):
+        torch.func.vmap(lambda t: dense.rms_norm_quant(t, w.new_ones(256).bfloat16())[1])(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", calls("cpu"))
+def test_gradients_are_never_lost_silently(name):
+    """As through torch.ops.strix: the result carries a node, whose backward pass warns."""
+    f, t = calls(DEV)[name]
+    want = f(t)
+    got = f(t.clone().requires_grad_())
+    assert torch.equal(got.detach(), want) and got.grad_fn is not None
+    with torch.no_grad():
+        assert not f(t.clone().requires_grad_()).requires_grad
