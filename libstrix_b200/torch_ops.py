@@ -1142,16 +1142,24 @@ def _same_device(first, *others) -> None:
         _check(t is None or t.get_device() == dev, "tensors must be on one device")
 
 
+# Not part of torch's public interface; None on a torch without them.
+_raw_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _launch(t, entry: str, *args) -> None:
     """Calls `entry` on t's device, its current stream the last argument. A decode step's
     smallest kernels take less time than a call of Python's device and stream objects
     (4.7 of a call's 26 us), hence the raw ones."""
     dev = t.get_device()
-    if dev == torch._C._cuda_getDevice():
-        _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(dev))
+    if _raw_device is None or _raw_stream is None:
+        with torch.cuda.device(dev):
+            _lib.call(entry, *args, torch.cuda.current_stream(dev).cuda_stream)
+    elif dev == _raw_device():
+        _lib.call(entry, *args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            _lib.call(entry, *args, torch._C._cuda_getCurrentRawStream(dev))
+            _lib.call(entry, *args, _raw_stream(dev))
 
 
 def _after_tcgen05(t, op: str) -> None:

@@ -3,12 +3,13 @@ a single row of any stride, non-finite and empty groups through each join of the
 product, strided operands there, overlapping streams, offsets beyond 32 bits. Bounds as
 in test_8bit_dense_layer.py."""
 
+import contextlib
 import warnings
 
 import pytest
 import torch
 
-from libstrix_b200 import dense
+from libstrix_b200 import dense, torch_ops
 from test_8bit_dense_layer import DEV, gemm_case, norm_case
 
 
@@ -58,6 +59,19 @@ def test_only_ordinary_calls_skip_the_dispatcher():
 def test_direct_path_needs_no_private_names(monkeypatch):
     monkeypatch.setattr(dense, "_are_functorch_transforms_active", None)
     assert not dense._plain(torch.randn(3))
+
+
+def test_launches_need_no_private_names(monkeypatch):
+    """Without torch's raw device and stream getters _launch uses the public objects."""
+    from types import SimpleNamespace
+
+    seen = []
+    monkeypatch.setattr(torch_ops, "_raw_stream", None)
+    monkeypatch.setattr(torch_ops._lib, "call", lambda *a: seen.append(a))
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext(seen.append(dev)))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev: SimpleNamespace(cuda_stream=77))
+    torch_ops._launch(SimpleNamespace(get_device=lambda: 3), "strix_entry", 1, 2)
+    assert seen == [3, ("strix_entry", 1, 2, 77)]
 
 
 @pytest.mark.parametrize("name", calls("cpu"))
