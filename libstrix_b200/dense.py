@@ -121,8 +121,10 @@ def fused_mlp_fp8_w8a8(x, norm_weight, w13, w13_scale, w2, w2_scale, eps: float 
 def fused_mlp_int8_w8a8(x, norm_weight, w13, w13_scale, w2, w2_scale, eps: float = 1e-6, residual=None,
                         residual_out=None, activation: str = "silu"):
     """The same block over int8 weights [2 I, H] and [H, I] with one fp32 scale per output
-    channel (H and I multiples of 128). Returns bf16 [T, H]."""
+    channel (H and I multiples of 128). Returns [T, H] of x's dtype. w8a8_int8_gemm rounds
+    to bf16, so under fp16 the increment has bf16's eight significant bits."""
     q, s = rms_norm_quant(x, norm_weight, eps, residual, residual_out, torch.int8)
     h = torch.ops.strix.w8a8_int8_gemm(q, s, w13, w13_scale)
     q, s = act_mul_quant(h, activation, torch.int8)
-    return torch.ops.strix.w8a8_int8_gemm(q, s, w2, w2_scale)
+    out = torch.ops.strix.w8a8_int8_gemm(q, s, w2, w2_scale)
+    return out if x.dtype == torch.bfloat16 else out.to(x.dtype)

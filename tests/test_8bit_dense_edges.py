@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from libstrix_b200 import dense, torch_ops
-from test_8bit_dense_layer import DEV, gemm_case, norm_case
+from test_8bit_dense_layer import DEV, F8, gemm_case, norm_case
 
 
 # ------------------------------------------------- transforms and derivatives
@@ -112,3 +112,40 @@ def test_gradients_are_never_lost_silently(name):
     assert torch.equal(got.detach(), want) and got.grad_fn is not None
     with torch.no_grad():
         assert not f(t.clone().requires_grad_()).requires_grad
+
+
+# ------------------------------------------------------------------ int8 MLP
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_mlp_blocks_return_the_type_of_their_rows(dtype):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def t(*shape, dtype):
+        return torch.empty(*shape, dtype=dtype, device="cuda")
+
+    f32, i8 = torch.float32, torch.int8
+    with FakeTensorMode():
+        x, w = t(3, 256, dtype=dtype), t(256, dtype=dtype)
+        out8 = dense.fused_mlp_int8_w8a8(x, w, t(768, 256, dtype=i8), t(768, dtype=f32), t(256, 384, dtype=i8),
+                                         t(256, dtype=f32))
+        outf = dense.fused_mlp_fp8_w8a8(x, w, t(768, 256, dtype=F8), t(6, 2, dtype=f32), t(256, 384, dtype=F8),
+                                        t(2, 3, dtype=f32))
+    assert out8.dtype == dtype and outf.dtype == dtype and out8.shape == outf.shape == (3, 256)
+
+
+@pytest.mark.gpu
+def test_int8_mlp_blocks_chain_in_fp16():
+    """The increment of one block is the next block's x, beside the residual stream."""
+    t, h, i = 19, 256, 384
+    x, r, w = norm_case(t, h, torch.float16, 3)
+    g = torch.Generator().manual_seed(4)
+    w13 = torch.randint(-127, 128, (2 * i, h), generator=g, dtype=torch.int8).to(DEV)
+    w2 = torch.randint(-127, 128, (h, i), generator=g, dtype=torch.int8).to(DEV)
+    s13, s2 = (torch.rand(2 * i, generator=g) * 1e-4 + 1e-4).to(DEV), (torch.rand(h, generator=g) * 1e-4).to(DEV)
+    xd, rd, wd = x.to(DEV), r.to(DEV), w.to(DEV)
+    y = dense.fused_mlp_int8_w8a8(xd, wd, w13, s13, w2, s2, residual=rd, residual_out=rd)
+    q, s = dense.rms_norm_quant(xd, wd, residual=r.to(DEV), q_dtype=torch.int8)
+    q, s = dense.act_mul_quant(torch.ops.strix.w8a8_int8_gemm(q, s, w13, s13), q_dtype=torch.int8)
+    assert torch.equal(y, torch.ops.strix.w8a8_int8_gemm(q, s, w2, s2).half())
+    dense.fused_mlp_int8_w8a8(y, wd, w13, s13, w2, s2, residual=rd, residual_out=rd)
+    want = ((x.float() + r.float()).half().float() + y.float().cpu()).half()
+    assert torch.equal(rd.cpu(), want)
