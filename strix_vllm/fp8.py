@@ -39,14 +39,19 @@ def apply_fp8_w8a8(x_2d: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
                    bias: torch.Tensor | None) -> torch.Tensor:
     """apply_fp8 for 128 x 128 block scales with 8-bit activations beyond 8 rows (up to
     there the weight stream sets the pace and the activations stay exact), and for the
-    widths that the W8A16 kernels do not take."""
+    widths that the W8A16 kernels do not take. A bias of another type than the kernels'
+    bf16 is added to fp32 sums (to the 16-bit ones up to 8 rows); the result is bf16."""
     x_2d = x_2d.contiguous()
+    own = bias is None or bias.dtype == torch.bfloat16
     if x_2d.size(0) <= 8 and w.size(0) % 16 == 0:
-        return apply_fp8(x_2d, w, scales, bias)
+        out = apply_fp8(x_2d, w, scales, bias if own else None)
+        return out if own else (out + bias).to(torch.bfloat16)
     from libstrix_b200 import dense, moe
 
     q, s = moe.act_quant_fp8(x_2d)
-    return dense.fp8_gemm(q, s, w, scales, None if bias is None else bias.contiguous(), torch.bfloat16)
+    if own:
+        return dense.fp8_gemm(q, s, w, scales, None if bias is None else bias.contiguous(), torch.bfloat16)
+    return dense.fp8_gemm(q, s, w, scales, bias.float().contiguous(), torch.float32).to(torch.bfloat16)
 
 
 def _apply_fake(x_2d, w, scales, bias):

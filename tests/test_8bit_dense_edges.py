@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from libstrix_b200 import dense, torch_ops
-from test_8bit_dense_layer import DEV, F8, gemm_case, norm_case
+from test_8bit_dense_layer import DEV, F8, gemm_case, norm_case, status_ok
 
 
 # ------------------------------------------------- transforms and derivatives
@@ -149,3 +149,43 @@ def test_int8_mlp_blocks_chain_in_fp16():
     dense.fused_mlp_int8_w8a8(y, wd, w13, s13, w2, s2, residual=rd, residual_out=rd)
     want = ((x.float() + r.float()).half().float() + y.float().cpu()).half()
     assert torch.equal(rd.cpu(), want)
+
+
+# ---------------------------------------------------------------- vLLM linear
+@pytest.mark.parametrize("rows", [3, 9])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_vllm_linear_hands_the_kernels_a_bias_of_their_type(monkeypatch, rows, dtype):
+    """With products that refuse what the kernels refuse, and add the bias as they do."""
+    from libstrix_b200 import moe
+    from strix_vllm import fp8
+
+    def product(q, s, w, scales, bias, out_dtype):
+        assert bias is None or bias.dtype == out_dtype and bias.is_contiguous()
+        out = torch.zeros(q.size(0), w.size(0)) if bias is None else bias.float().expand(q.size(0), -1)
+        return out.to(out_dtype)
+
+    def few(x, w, scales, bias):
+        assert bias is None or bias.dtype == torch.bfloat16
+        return product(x, None, w, scales, bias, torch.bfloat16)
+
+    monkeypatch.setattr(moe, "act_quant_fp8", lambda x: (x, None))
+    monkeypatch.setattr(dense, "fp8_gemm", product)
+    monkeypatch.setattr(fp8, "apply_fp8", few)
+    bias = torch.randn(64)[::2].to(dtype)
+    out = fp8.apply_fp8_w8a8(torch.zeros(rows, 128).bfloat16(), torch.zeros(32, 128), torch.zeros(1, 1), bias)
+    assert out.dtype == torch.bfloat16 and torch.equal(out, bias.bfloat16().expand(rows, -1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 9, 100])
+def test_vllm_linear_with_an_fp32_bias(rows):
+    from strix_vllm import fp8
+
+    x = norm_case(rows, 640, torch.bfloat16, 30, False)[0].to(DEV)
+    w, sw = (t.to(DEV) for t in gemm_case(1, 384, 640, 31)[2:])
+    bias = torch.randn(384, generator=torch.Generator().manual_seed(5)).to(DEV)
+    out, bare = fp8.apply_fp8_w8a8(x, w, sw, bias), fp8.apply_fp8_w8a8(x, w, sw, None)
+    status_ok()
+    want = bare.double() + bias.double()
+    # half a step of the 16-bit sums, and half a step of the result
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -8) * (bare.double().abs() + want.abs())).all()
