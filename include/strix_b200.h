@@ -242,8 +242,8 @@ int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, const float* a
  * [rows] (s_stride apart) = amax / 127, k a multiple of 8. A scale below the smallest
  * normal number (an all-zero group) is 1; q = y / scale to nearest even; a NaN or an
  * infinity in a group shows in its scale. x, residual bf16 (fp16 if in_f16), weight
- * of the same type or fp32 (weight_f32); element strides, rows on 16-byte boundaries,
- * k at most 65,536. vLLM's norm does this step in the reference's deployment, in
+ * of the same type or fp32 (weight_f32); element strides (of a single row they are not
+ * read), rows on 16-byte boundaries, k at most 65,536. vLLM's norm does this step in the reference's deployment, in
  * 16 bits; its GEMMs quantise (csrc/gemm/w8a8_wmma_gemm.hip:508-529). */
 int strix_rms_norm_quant(const void* x, const void* residual, void* residual_out, const void* weight,
                          void* q, float* scales, int64_t rows, int64_t k, int64_t x_stride,

@@ -397,13 +397,14 @@ extern "C" int strix_rms_norm_quant(const void* x, const void* residual, void* r
   STRIX_CHECK(rows < (int64_t(1) << 31), "too many rows");
   STRIX_CHECK(x != nullptr && weight != nullptr && q != nullptr && scales != nullptr, "pointers must not be NULL");
   STRIX_CHECK(residual_out == nullptr || residual != nullptr, "residual_out needs a residual");
+  // a single row's strides are not read: any will do
+  if (rows == 1) x_stride = r_stride = ro_stride = q_stride = k, s_stride = (k + 127) / 128;
   STRIX_CHECK(aligned(x, 16) && aligned(residual, 16) && aligned(residual_out, 16) && aligned(weight, 16) &&
                   aligned(q, 8) && x_stride % 8 == 0 && r_stride % 8 == 0 && ro_stride % 8 == 0 &&
                   q_stride % 8 == 0,
               "16-byte aligned rows required");
-  STRIX_CHECK(x_stride >= 0 && r_stride >= 0 && q_stride >= (rows > 1 ? k : 0) &&
-                  s_stride >= (rows > 1 ? (fp8 ? (k + 127) / 128 : 1) : 0) &&
-                  (residual_out == nullptr || rows == 1 || ro_stride >= k),
+  STRIX_CHECK(x_stride >= 0 && r_stride >= 0 && q_stride >= k && s_stride >= (fp8 ? (k + 127) / 128 : 1) &&
+                  (residual_out == nullptr || ro_stride >= k),
               "output rows must not overlap");
   if (residual_out != nullptr) {
     // a row is read whole before any of it is written, so the sum may replace x or the
@@ -442,10 +443,11 @@ extern "C" int strix_act_mul_quant(const void* x, void* q, float* scales, int64_
   if (rows == 0) return STRIX_OK;
   STRIX_CHECK(rows < (int64_t(1) << 31) && rows * ((k + 127) / 128) < (int64_t(1) << 31) - 64, "too many rows");
   STRIX_CHECK(x != nullptr && q != nullptr && scales != nullptr, "pointers must not be NULL");
+  // a single row's strides are not read: any will do
+  if (rows == 1) x_stride = 2 * k, q_stride = k, s_stride = (k + 127) / 128;
   STRIX_CHECK(aligned(x, 16) && aligned(q, 8) && x_stride % (in_type == 2 ? 4 : 8) == 0 && q_stride % 8 == 0,
               "16-byte aligned rows required");
-  STRIX_CHECK(x_stride >= 0 && q_stride >= (rows > 1 ? k : 0) &&
-                  s_stride >= (rows > 1 ? (fp8 ? (k + 127) / 128 : 1) : 0),
+  STRIX_CHECK(x_stride >= 0 && q_stride >= k && s_stride >= (fp8 ? (k + 127) / 128 : 1),
               "output rows must not overlap");
   ActArgs p;
   p.x = x, p.q = static_cast<uint8_t*>(q), p.scales = scales;

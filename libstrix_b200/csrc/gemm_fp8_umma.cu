@@ -955,8 +955,9 @@ extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, con
   int rc = fp8_operands(p, a_q, a_scale, w, w_scale, m, 2 * n, k, a_stride, w_stride, dev, sms);
   if (rc != STRIX_OK || m == 0) return rc;
   STRIX_CHECK(q != nullptr && scales != nullptr, "pointers must not be NULL");
+  if (m == 1) q_stride = n, s_stride = (n + 127) / 128;   // not read: any will do
   STRIX_CHECK(reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride % 16 == 0, "16-byte aligned rows required");
-  STRIX_CHECK(m == 1 || (q_stride >= n && s_stride >= (n + 127) / 128), "output rows must not overlap");
+  STRIX_CHECK(q_stride >= n && s_stride >= (n + 127) / 128, "output rows must not overlap");
   p.sa_sm = sa_stride_m, p.sa_sk = sa_stride_k, p.sw_sn = sw_stride_n, p.sw_sk = sw_stride_k;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (gated_in_one(n)) {

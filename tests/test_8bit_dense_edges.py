@@ -189,3 +189,48 @@ def test_vllm_linear_with_an_fp32_bias(rows):
     want = bare.double() + bias.double()
     # half a step of the 16-bit sums, and half a step of the result
     assert ((out.double() - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -8) * (bare.double().abs() + want.abs())).all()
+
+
+# ------------------------------------------------------- strides of one element
+def odd_row(t):
+    """The row t [1, K] with a row stride that no kernel could walk."""
+    return t.as_strided(t.shape, (t.size(1) + 3, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_dtype", [F8, torch.int8])
+def test_a_single_row_may_have_any_stride(q_dtype):
+    x, r, w = (t.to(DEV) for t in norm_case(1, 256, torch.bfloat16, 6))
+    wide = torch.zeros(1, 261, dtype=x.dtype, device=DEV)        # a slice of a matrix of odd width
+    wide[:, :256] = x
+    want = dense.rms_norm_quant(x, w, residual=r, q_dtype=q_dtype)
+    for xx, rr in ((odd_row(x), r), (x, odd_row(r)), (wide[:, :256], odd_row(r)), (x.as_strided((1, 256), (1, 1)), r)):
+        out = odd_row(torch.empty_like(r))
+        got = dense.rms_norm_quant(xx, w, residual=rr, residual_out=out, q_dtype=q_dtype)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+        assert torch.equal(out, (x.float() + r.float()).bfloat16())
+    in_place = x.clone()                                         # x itself, under two strides
+    dense.rms_norm_quant(in_place, w, residual=r, residual_out=odd_row(in_place), q_dtype=q_dtype)
+    assert torch.equal(in_place, (x.float() + r.float()).bfloat16())
+    with pytest.raises(RuntimeError, match="apart"):             # half of it stays refused
+        both = torch.zeros(1, 512, dtype=x.dtype, device=DEV)
+        dense.rms_norm_quant(both[:, :256], w, residual=r, residual_out=both[:, 128:384], q_dtype=q_dtype)
+    want = dense.act_mul_quant(x, q_dtype=q_dtype)
+    for xx in (odd_row(x), wide[:, :256]):
+        got = dense.act_mul_quant(xx, q_dtype=q_dtype)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [256, 144])
+def test_a_single_row_of_the_gated_product_may_have_any_stride(n):
+    """The C entry, with output strides that only more rows would need."""
+    k = 256
+    a, sa, w, sw = (t.to(DEV) for t in gemm_case(1, 2 * n, k, 7))
+    q, s = dense.fp8_gemm_act_mul_quant(a, sa, w, sw)
+    q2, s2 = torch.empty_like(q), torch.empty_like(s)
+    ws = torch.empty(2 * n * 4, dtype=torch.uint8, device=DEV)
+    torch_ops._launch(a, "strix_w8a8_fp8_gated", q2.data_ptr(), s2.data_ptr(), a.data_ptr(), sa.data_ptr(), w.data_ptr(),
+                      sw.data_ptr(), ws.data_ptr(), ws.numel(), 1, n, k, 7, k, 5, 0, *sa.stride(), *sw.stride(), 1)
+    status_ok()
+    assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s, s2)
