@@ -1307,7 +1307,7 @@ def w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=None):
     _check(kind is not None, "out_dtype must be bf16, fp16 or fp32")
     bias_ptr = None
     if bias is not None:
-        _check(bias.dtype is out_dtype and bias.shape == (n,) and bias.stride() == (1,),
+        _check(bias.dtype is out_dtype and bias.shape == (n,) and bias.is_contiguous(),
                "bias must be contiguous [N] of the output's dtype")
         _same_device(a_q, bias)
         bias_ptr = bias.data_ptr()

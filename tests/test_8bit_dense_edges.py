@@ -234,3 +234,10 @@ def test_a_single_row_of_the_gated_product_may_have_any_stride(n):
                       sw.data_ptr(), ws.data_ptr(), ws.numel(), 1, n, k, 7, k, 5, 0, *sa.stride(), *sw.stride(), 1)
     status_ok()
     assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s, s2)
+
+
+@pytest.mark.gpu
+def test_a_bias_of_one_element_may_have_any_stride():
+    a, sa, w, sw = (t.to(DEV) for t in gemm_case(5, 1, 256, 8))
+    bias = torch.randn(6, device=DEV).bfloat16()
+    assert torch.equal(dense.fp8_gemm(a, sa, w, sw, bias[::6]), dense.fp8_gemm(a, sa, w, sw, bias[:1].clone()))
