@@ -319,10 +319,15 @@ int device_sms(int& dev, int& sms) {
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
-// Whether [a, a + a_bytes) and [b, b + b_bytes) share a byte.
-bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+// Whether two matrices of `rows` rows of `width` bytes, the row strides in bytes, may share
+// a byte. Rows side by side in one wider matrix (slices of its columns) do not.
+bool overlap(const void* a, int64_t a_st, const void* b, int64_t b_st, int64_t rows, int64_t width) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + uintptr_t(b_bytes) && y < x + uintptr_t(a_bytes);
+  const uintptr_t a_end = x + uintptr_t((rows - 1) * a_st + width), b_end = y + uintptr_t((rows - 1) * b_st + width);
+  if (x >= b_end || y >= a_end) return false;
+  if (a_st != b_st || a_st < 2 * width) return true;
+  const int64_t apart = int64_t((x > y ? x - y : y - x) % uintptr_t(a_st));
+  return apart < width || apart > a_st - width;
 }
 
 template <bool F8, bool F16, bool WF32, int V>
@@ -409,12 +414,11 @@ extern "C" int strix_rms_norm_quant(const void* x, const void* residual, void* r
   if (residual_out != nullptr) {
     // a row is read whole before any of it is written, so the sum may replace x or the
     // residual in place; any other overlap would let one row's sum into another's input
-    const int64_t out_bytes = ((rows - 1) * ro_stride + k) * 2;
     STRIX_CHECK((residual_out == x && ro_stride == x_stride) ||
-                    !overlap(residual_out, out_bytes, x, ((rows - 1) * x_stride + k) * 2),
+                    !overlap(residual_out, ro_stride * 2, x, x_stride * 2, rows, k * 2),
                 "residual_out must be x itself or apart from it");
     STRIX_CHECK((residual_out == residual && ro_stride == r_stride) ||
-                    !overlap(residual_out, out_bytes, residual, ((rows - 1) * r_stride + k) * 2),
+                    !overlap(residual_out, ro_stride * 2, residual, r_stride * 2, rows, k * 2),
                 "residual_out must be residual itself or apart from it");
   }
   NormArgs p;

@@ -241,3 +241,38 @@ def test_a_bias_of_one_element_may_have_any_stride():
     a, sa, w, sw = (t.to(DEV) for t in gemm_case(5, 1, 256, 8))
     bias = torch.randn(6, device=DEV).bfloat16()
     assert torch.equal(dense.fp8_gemm(a, sa, w, sw, bias[::6]), dense.fp8_gemm(a, sa, w, sw, bias[:1].clone()))
+
+
+# ------------------------------------------------------ slices of one wider matrix
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_dtype", [F8, torch.int8])
+def test_norm_with_rows_side_by_side_in_one_matrix(q_dtype):
+    m, k = 9, 256
+    x, r, w = (t.to(DEV) for t in norm_case(m, k, torch.bfloat16, 9))
+    want = dense.rms_norm_quant(x, w, residual=r, q_dtype=q_dtype)
+    total = (x.float() + r.float()).bfloat16()
+    for at_x, at_r, at_out in ((0, 256, 512), (512, 0, 256), (264, 520, 8)):
+        wide = torch.full((m, 3 * k + 8), -7.0, dtype=x.dtype, device=DEV)
+        wide[:, at_x:at_x + k], wide[:, at_r:at_r + k] = x, r
+        out = wide[:, at_out:at_out + k]
+        got = dense.rms_norm_quant(wide[:, at_x:at_x + k], w, residual=wide[:, at_r:at_r + k], residual_out=out,
+                                   q_dtype=q_dtype)
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+        assert torch.equal(out, total)
+        assert torch.equal(wide[:, at_x:at_x + k], x) and torch.equal(wide[:, at_r:at_r + k], r)
+        assert ((wide == -7.0).sum() >= 8 * m).item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [8, 248, 264, 504, 776, 1016])
+def test_norm_refuses_a_sum_that_runs_into_its_input(first):
+    """Columns [256, 512) of rows of 768 as input: a sum that starts less than a row's
+    width before or behind them, in the same row or the next one."""
+    buf = torch.zeros(4 * 768 + 1024, dtype=torch.bfloat16, device=DEV)
+    x = buf.as_strided((4, 256), (768, 1), 256)
+    out = buf.as_strided((4, 256), (768, 1), first)
+    r, w = torch.ones(4, 256, device=DEV).bfloat16(), torch.ones(256, device=DEV).bfloat16()
+    with pytest.raises(RuntimeError, match="apart"):
+        dense.rms_norm_quant(x, w, residual=r, residual_out=out)
+    with pytest.raises(RuntimeError, match="apart"):
+        dense.rms_norm_quant(r, w, residual=x, residual_out=out)
