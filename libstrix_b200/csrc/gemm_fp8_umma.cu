@@ -817,9 +817,6 @@ int launch_wide(Fp8GemmArgs p, int splits, const void* a, int64_t a_st, const vo
                   tma::make_map_u8(&map_a, a, uint64_t(p.M), uint64_t(k), uint64_t(a_st), 128) &&
                   (!p.tma_out || tma::make_map_u8(&map_o, p.out, uint64_t(p.M), uint64_t(p.N) * bytes, uint64_t(o_st), 32)),
               "tensor map encoding failed");
-#ifdef WSPL
-  splits = WSPL;
-#endif
   p.splits = splits;
   const int64_t pairs = splits > 1 || tiles < sms / 2 ? tiles * splits : sms / 2;
   STRIX_CUDA(cluster::launch(kernel, unsigned(2 * pairs), unsigned(2 * splits), kWideThreads, L::kSmem, st, p, map_w, map_a, map_o));

@@ -4,7 +4,9 @@ product, strided operands there, overlapping streams, offsets beyond 32 bits. Bo
 in test_8bit_dense_layer.py."""
 
 import contextlib
+import re
 import warnings
+from pathlib import Path
 
 import pytest
 import torch
@@ -276,3 +278,13 @@ def test_norm_refuses_a_sum_that_runs_into_its_input(first):
         dense.rms_norm_quant(x, w, residual=r, residual_out=out)
     with pytest.raises(RuntimeError, match="apart"):
         dense.rms_norm_quant(r, w, residual=x, residual_out=out)
+
+
+# -------------------------------------------------------------------- the build
+def test_kernel_sources_have_no_switches():
+    """What the kernels do is chosen by sizes, types and alignment at run time: no part of a
+    source is compiled in or out."""
+    csrc = Path(dense.__file__).parent / "csrc"
+    found = [f"{f.name}:{i}" for f in sorted(csrc.iterdir()) for i, line in enumerate(f.read_text().splitlines(), 1)
+             if re.match(r"\s*#\s*(if|ifdef|ifndef|elif)\b", line)]
+    assert not found
