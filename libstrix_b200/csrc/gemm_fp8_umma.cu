@@ -34,7 +34,7 @@ struct Fp8GemmArgs {
   int32_t* status;
   int64_t out_st, sa_sm, sa_sk, sw_sn, sw_sk;
   int M, N, nkb;
-  int n_tiles, splits;             // stream kernel: 128-row weight tiles, CTAs per tile along K
+  int n_tiles, splits;             // wide kernel: tiles of BN weight rows; CTAs, or pairs of them, per tile along K
   // gated form: `out` holds the e4m3 rows, N counts gate and up rows together
   float* q_scales;                 // [M, N / 256], row stride qs_st
   int64_t qs_st;
@@ -101,8 +101,7 @@ __global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayou
   __shared__ volatile int s_abort;
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  const int rank = int(blockIdx.x) % p.splits, tile = int(blockIdx.x) / p.splits;
-  const int n0 = (tile % p.n_tiles) * 128, m0 = (tile / p.n_tiles) * NB;
+  const int rank = int(blockIdx.x) % p.splits, n0 = int(blockIdx.x) / p.splits * 128;
   // K blocks [k0, k0 + nk) of this CTA
   const int base = p.nkb / p.splits, rem = p.nkb % p.splits;
   const int nk = base + (rank < rem ? 1 : 0), k0 = rank * base + min(rank, rem);
@@ -142,7 +141,7 @@ __global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayou
         tma::mbar_expect_tx(&full_bar[s], L::kStageBytes);
         tma::load_2d(st, &map_w, (k0 + t) * kBlk, n0, &full_bar[s]);
         if constexpr (GATED) tma::load_2d(st + 128 * kBlk, &map_w, (k0 + t) * kBlk, p.N / 2 + n0, &full_bar[s]);
-        tma::load_2d(st + L::kWBytes, &map_a, (k0 + t) * kBlk, m0, &full_bar[s]);
+        tma::load_2d(st + L::kWBytes, &map_a, (k0 + t) * kBlk, 0, &full_bar[s]);
       }
       __syncwarp();
       if (++s == S) s = 0, ph ^= 1;
@@ -188,9 +187,9 @@ __global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayou
         break;
       }
       for (int j = lane; j < NB; j += 32) {
-        const bool live = m0 + j < p.M;
+        const bool live = j < p.M;
         cp_async_4_zfill(smem_u32(s_scale + s * NB + j),
-                         p.sa + (live ? int64_t(m0 + j) * p.sa_sm + int64_t(k0 + t) * p.sa_sk : 0), live);
+                         p.sa + (live ? int64_t(j) * p.sa_sm + int64_t(k0 + t) * p.sa_sk : 0), live);
       }
       mbar_arrive_cp_async(&sfull_bar[s]);
       if (++s == S) s = 0, ph ^= 1;
@@ -263,7 +262,7 @@ __global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayou
       const float bias = load_bias(p.bias, p.out_kind, n);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
-        if (m0 + j < p.M) store_one(p.out, p.out_kind, int64_t(m0 + j) * p.out_st + n, acc[j] + bias);
+        if (j < p.M) store_one(p.out, p.out_kind, int64_t(j) * p.out_st + n, acc[j] + bias);
     }
     return;
   }
@@ -292,9 +291,9 @@ __global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayou
     __shared__ float s_amax[2][G][4];
     int par = 0;
     // all threads take the same rounds: they meet at a barrier in each
-    for (int j0 = rank * G; j0 < NB && m0 + j0 < p.M; j0 += G * p.splits, par ^= 1) {
+    for (int j0 = rank * G; j0 < p.M; j0 += G * p.splits, par ^= 1) {
       const int j = j0 + grp;
-      const bool live = j < NB && m0 + j < p.M;
+      const bool live = j < p.M;
       float y = 0.f;
       if (live) y = quant8::gate(joined(j), p.gate_act) * joined(NB + j);
       float amax = fabsf(y);
@@ -305,25 +304,26 @@ __global__ void __launch_bounds__(StreamLayout<NB, GATED>::kThreads, StreamLayou
       const float* a4 = s_amax[par][grp];
       const float sc = quant8::scale_of(quant8::max_nan(quant8::max_nan(a4[0], a4[1], a4[2]), a4[3]), quant8::kTopF8);
       if (live) {
-        static_cast<uint8_t*>(p.out)[int64_t(m0 + j) * p.out_st + col] =
+        static_cast<uint8_t*>(p.out)[int64_t(j) * p.out_st + col] =
             uint8_t(quant8::pack_e4m3x4(y * quant8::rcp(sc), 0.f, 0.f, 0.f));
-        if (row == 0) p.q_scales[int64_t(m0 + j) * p.qs_st + n0 / kBlk] = sc;
+        if (row == 0) p.q_scales[int64_t(j) * p.qs_st + n0 / kBlk] = sc;
       }
     }
   } else {
     const float bias = col < p.N ? load_bias(p.bias, p.out_kind, col) : 0.f;
-    for (int j = rank * G + grp; j < NB && m0 + j < p.M; j += G * p.splits) {
+    for (int j = rank * G + grp; j < p.M; j += G * p.splits) {
       const float v = joined(j);
-      if (col < p.N) store_one(p.out, p.out_kind, int64_t(m0 + j) * p.out_st + col, v + bias);
+      if (col < p.N) store_one(p.out, p.out_kind, int64_t(j) * p.out_st + col, v + bias);
     }
   }
   cluster::sync();   // nobody leaves while a peer still reads its shared memory
 }
 
 template <int NB, bool GATED>
-int launch_stream(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
-                  int dev, cudaStream_t st) {
+int launch_stream(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int dev,
+                  cudaStream_t st) {
   using L = StreamLayout<NB, GATED>;
+  STRIX_CHECK(p.M <= NB, "the weight stream takes up to %d tokens here", NB);
   auto kernel = gemm_fp8_stream_kernel<NB, GATED>;
   static int places[64][kMaxSplits + 1] = {};   // clusters of c CTAs that find an SM each (asked once)
   if (!places[dev][1]) {
@@ -331,8 +331,7 @@ int launch_stream(Fp8GemmArgs p, const void* a, int64_t a_st, const void* w, int
     for (int c = kMaxSplits; c >= 1; --c)
       STRIX_CUDA(cluster::places(&places[dev][c], kernel, unsigned(c), unsigned(L::kThreads), L::kSmem));
   }
-  p.n_tiles = GATED ? p.N / 256 : (p.N + 127) / 128;
-  const int64_t tiles = int64_t(p.n_tiles) * ((p.M + NB - 1) / NB);
+  const int64_t tiles = GATED ? p.N / 256 : (p.N + 127) / 128;
   // As many CTAs per tile as leave each two K blocks and every cluster a place at once: a
   // second round costs more than shorter CTAs give. Measured on 16 x 5,120 x 17,408 (40
   // tiles; clusters of 6 are the largest that all fit): 36.8, 22.7, 20.0, 19.2, 18.7, 18.8,
@@ -897,9 +896,9 @@ int fp8_operands(Fp8GemmArgs& p, const void* a_q, const float* a_scale, const vo
 
 int run_gemm(const Fp8GemmArgs& p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
              int dev, cudaStream_t st) {
-  if (p.M <= 16) return launch_stream<16, false>(p, a, a_st, w, w_st, k, sms, dev, st);
-  if (p.M <= 32) return launch_stream<32, false>(p, a, a_st, w, w_st, k, sms, dev, st);
-  if (p.M <= 64) return launch_stream<64, false>(p, a, a_st, w, w_st, k, sms, dev, st);
+  if (p.M <= 16) return launch_stream<16, false>(p, a, a_st, w, w_st, k, dev, st);
+  if (p.M <= 32) return launch_stream<32, false>(p, a, a_st, w, w_st, k, dev, st);
+  if (p.M <= 64) return launch_stream<64, false>(p, a, a_st, w, w_st, k, dev, st);
   const int* places = nullptr;
   const int rc = pair_places(dev, &places);
   if (rc != STRIX_OK) return rc;
@@ -961,8 +960,8 @@ extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, con
     // (33 to 64 tokens: the weight stream took 40.0 and 44.9 us at 33 and 64 x 17,408 x 5,120, the
     // wide tiles 42.9 and 43.3)
     p.out = q, p.out_st = q_stride, p.q_scales = scales, p.qs_st = s_stride, p.gate_act = gate_act;
-    if (m <= 16) return launch_stream<16, true>(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
-    if (m <= 32) return launch_stream<32, true>(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
+    if (m <= 16) return launch_stream<16, true>(p, a_q, a_stride, w, w_stride, k, dev, st);
+    if (m <= 32) return launch_stream<32, true>(p, a_q, a_stride, w, w_stride, k, dev, st);
     const int* places = nullptr;
     rc = pair_places(dev, &places);
     if (rc != STRIX_OK) return rc;
