@@ -792,9 +792,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) gemm_fp8_wide_kernel(
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
+// `room`: pairs that find a place at once. Tiles go to the pairs by turns, so a pair beyond
+// that would begin its share when another has ended its own.
 template <int BN, bool GATED>
-int launch_wide(Fp8GemmArgs p, int splits, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k,
-                int sms, int dev, cudaStream_t st) {
+int launch_wide(Fp8GemmArgs p, int splits, int64_t room, const void* a, int64_t a_st, const void* w, int64_t w_st,
+                int64_t k, int dev, cudaStream_t st) {
   using L = WideLayout<BN>;
   auto kernel = gemm_fp8_wide_kernel<BN, GATED>;
   static bool done[64] = {};
@@ -817,7 +819,7 @@ int launch_wide(Fp8GemmArgs p, int splits, const void* a, int64_t a_st, const vo
                   (!p.tma_out || tma::make_map_u8(&map_o, p.out, uint64_t(p.M), uint64_t(p.N) * bytes, uint64_t(o_st), 32)),
               "tensor map encoding failed");
   p.splits = splits;
-  const int64_t pairs = splits > 1 || tiles < sms / 2 ? tiles * splits : sms / 2;
+  const int64_t pairs = splits > 1 || tiles < room ? tiles * splits : room;
   STRIX_CUDA(cluster::launch(kernel, unsigned(2 * pairs), unsigned(2 * splits), kWideThreads, L::kSmem, st, p, map_w, map_a, map_o));
   return launch_status("w8a8_fp8_gemm");
 }
@@ -866,7 +868,7 @@ WidePlan wide_plan(int64_t m, int64_t n, int nkb, bool gated, const int* places)
 
 // The checks that both entry points share; fills what the kernels read of the operands.
 int fp8_operands(Fp8GemmArgs& p, const void* a_q, const float* a_scale, const void* w, const float* w_scale,
-                 int64_t m, int64_t n, int64_t k, int64_t& a_stride, int64_t& w_stride, int& dev, int& sms) {
+                 int64_t m, int64_t n, int64_t k, int64_t& a_stride, int64_t& w_stride, int& dev) {
   STRIX_CHECK(m >= 0 && n > 0 && k > 0, "bad shapes");
   STRIX_CHECK(k % 16 == 0, "K must be a multiple of 16");
   STRIX_CHECK(n < (int64_t(1) << 31) - 256 && m < (int64_t(1) << 31) - 256 && k < (int64_t(1) << 31) - 256,
@@ -886,16 +888,13 @@ int fp8_operands(Fp8GemmArgs& p, const void* a_q, const float* a_scale, const vo
   p.status = umma_status_ptr();
   STRIX_CHECK(p.status != nullptr, "status word unavailable");
   p.M = int(m), p.N = int(n), p.nkb = int((k + kBlk - 1) / kBlk);
-  static int sm_count[64] = {};
   STRIX_CUDA(cudaGetDevice(&dev));
   STRIX_CHECK(dev >= 0 && dev < 64, "device index %d out of range", dev);
-  if (!sm_count[dev]) STRIX_CUDA(cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev));
-  sms = sm_count[dev];
   return STRIX_OK;
 }
 
-int run_gemm(const Fp8GemmArgs& p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int sms,
-             int dev, cudaStream_t st) {
+int run_gemm(const Fp8GemmArgs& p, const void* a, int64_t a_st, const void* w, int64_t w_st, int64_t k, int dev,
+             cudaStream_t st) {
   if (p.M <= 16) return launch_stream<16, false>(p, a, a_st, w, w_st, k, dev, st);
   if (p.M <= 32) return launch_stream<32, false>(p, a, a_st, w, w_st, k, dev, st);
   if (p.M <= 64) return launch_stream<64, false>(p, a, a_st, w, w_st, k, dev, st);
@@ -903,8 +902,8 @@ int run_gemm(const Fp8GemmArgs& p, const void* a, int64_t a_st, const void* w, i
   const int rc = pair_places(dev, &places);
   if (rc != STRIX_OK) return rc;
   const WidePlan plan = wide_plan(p.M, p.N, p.nkb, false, places);
-  if (plan.bn == 128) return launch_wide<128, false>(p, plan.splits, a, a_st, w, w_st, k, sms, dev, st);
-  return launch_wide<256, false>(p, plan.splits, a, a_st, w, w_st, k, sms, dev, st);
+  if (plan.bn == 128) return launch_wide<128, false>(p, plan.splits, places[1], a, a_st, w, w_st, k, dev, st);
+  return launch_wide<256, false>(p, plan.splits, places[1], a, a_st, w, w_st, k, dev, st);
 }
 
 }  // namespace
@@ -919,14 +918,14 @@ extern "C" int strix_w8a8_fp8_gemm(void* out, const void* a_q, const float* a_sc
                                    int64_t sw_stride_k, int out_kind, strix_stream_t stream) {
   STRIX_CHECK(out_kind >= 0 && out_kind <= 2, "output must be bf16, fp16 or fp32");
   Fp8GemmArgs p{};
-  int dev = 0, sms = 0;
-  const int rc = fp8_operands(p, a_q, a_scale, w, w_scale, m, n, k, a_stride, w_stride, dev, sms);
+  int dev = 0;
+  const int rc = fp8_operands(p, a_q, a_scale, w, w_scale, m, n, k, a_stride, w_stride, dev);
   if (rc != STRIX_OK || m == 0) return rc;
   STRIX_CHECK(out != nullptr && (m == 1 || out_stride >= n), "output rows must not overlap");
   p.out = out, p.bias = bias, p.out_kind = out_kind;
   p.out_st = out_stride, p.sa_sm = sa_stride_m, p.sa_sk = sa_stride_k;
   p.sw_sn = sw_stride_n, p.sw_sk = sw_stride_k;
-  return run_gemm(p, a_q, a_stride, w, w_stride, k, sms, dev, static_cast<cudaStream_t>(stream));
+  return run_gemm(p, a_q, a_stride, w, w_stride, k, dev, static_cast<cudaStream_t>(stream));
 }
 
 // Whether the gated product runs in one kernel. Otherwise (gate and up rows that share a
@@ -947,8 +946,8 @@ extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, con
   STRIX_CHECK(gate_act == 1 || gate_act == 2, "activation must be silu or gelu_tanh");
   STRIX_CHECK(n > 0 && n < (int64_t(1) << 30) - 128 && n % 16 == 0, "N must be a multiple of 16");
   Fp8GemmArgs p{};
-  int dev = 0, sms = 0;
-  int rc = fp8_operands(p, a_q, a_scale, w, w_scale, m, 2 * n, k, a_stride, w_stride, dev, sms);
+  int dev = 0;
+  int rc = fp8_operands(p, a_q, a_scale, w, w_scale, m, 2 * n, k, a_stride, w_stride, dev);
   if (rc != STRIX_OK || m == 0) return rc;
   STRIX_CHECK(q != nullptr && scales != nullptr, "pointers must not be NULL");
   if (m == 1) q_stride = n, s_stride = (n + 127) / 128;   // not read: any will do
@@ -966,13 +965,13 @@ extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, con
     rc = pair_places(dev, &places);
     if (rc != STRIX_OK) return rc;
     const int splits = wide_plan(m, 2 * n, p.nkb, true, places).splits;
-    return launch_wide<256, true>(p, splits, a_q, a_stride, w, w_stride, k, sms, dev, st);
+    return launch_wide<256, true>(p, splits, places[1], a_q, a_stride, w, w_stride, k, dev, st);
   }
   const int64_t need = m * 2 * n * 4;
   STRIX_CHECK(workspace_bytes >= need && workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
               "workspace must hold %lld bytes on a 16-byte boundary", (long long)need);
   p.out = workspace, p.out_kind = kOutF32, p.out_st = 2 * n;
-  rc = run_gemm(p, a_q, a_stride, w, w_stride, k, sms, dev, st);
+  rc = run_gemm(p, a_q, a_stride, w, w_stride, k, dev, st);
   if (rc != STRIX_OK) return rc;
   return strix_act_mul_quant(workspace, q, scales, m, n, 2 * n, q_stride, s_stride, gate_act, 2, 1, stream);
 }
