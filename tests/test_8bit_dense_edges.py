@@ -12,7 +12,8 @@ import pytest
 import torch
 
 from libstrix_b200 import dense, torch_ops
-from test_8bit_dense_layer import DEV, F8, gemm_case, norm_case, status_ok
+from oracle import dense as O
+from test_8bit_dense_layer import DEV, F8, GATE_REL, check_rows, gemm_case, gemm_error, norm_case, status_ok
 
 
 # ------------------------------------------------- transforms and derivatives
@@ -278,6 +279,141 @@ def test_norm_refuses_a_sum_that_runs_into_its_input(first):
         dense.rms_norm_quant(x, w, residual=r, residual_out=out)
     with pytest.raises(RuntimeError, match="apart"):
         dense.rms_norm_quant(r, w, residual=x, residual_out=out)
+
+
+# ------------------------------------------------------------- gated product's joins
+# One shape per way that the sums reach the gate: the weight stream's join (two tile
+# widths), the wide kernel's registers and its join along K, and fp32 rows through the
+# workspace (gate and up rows that share a weight block) from either kernel.
+JOINS = {
+    "stream16": (9, 384, 656),
+    "stream32": (20, 384, 4112),
+    "wide": (70, 384, 640),
+    "wide_split": (70, 256, 6016),
+    "rows_stream": (9, 144, 656),
+    "rows_wide": (70, 400, 640),
+}
+
+
+def gated_case(join, seed):
+    m, n, k = JOINS[join]
+    a, sa, w, sw = gemm_case(m, 2 * n, k, seed)
+    return m, n, k, a, sa * 0.03, w, sw
+
+
+def gated(a, sa, w, sw, activation="silu"):
+    q, s = dense.fp8_gemm_act_mul_quant(a.to(DEV), sa.to(DEV), w.to(DEV), sw.to(DEV), activation)
+    status_ok()
+    return q.cpu().view(torch.uint8), s.cpu()
+
+
+def same_outside(got, want, rows=None, group=None):
+    """Equal to the bit except in the given rows, or in one group of 128 columns."""
+    keep = torch.ones(want[1].shape, dtype=torch.bool)
+    if rows is not None:
+        keep[rows] = False
+    if group is not None:
+        keep[:, group] = False
+    wide = O.spread(keep, want[0].size(1), 128)
+    return torch.equal(got[1][keep], want[1][keep]) and torch.equal(got[0][wide], want[0][wide])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("join", JOINS)
+def test_gated_product_shows_nan_and_infinity_where_they_are(join, activation):
+    m, n, k, a, sa, w, sw = gated_case(join, 70)
+    want = gated(a, sa, w, sw, activation)
+    bad = a.clone()
+    bad.view(torch.uint8)[1, 300] = 0x7F                 # a NaN in a token: its row, every group
+    got = gated(bad, sa, w, sw, activation)
+    assert got[1][1].isnan().all() and same_outside(got, want, rows=[1])
+    for row, group in ((130, 1), (n + 5, 0)):            # in a gate row, in an up row: its group
+        bad = w.clone()
+        bad.view(torch.uint8)[row, k - 1] = 0x7F
+        got = gated(a, sa, bad, sw, activation)
+        assert got[1][:, group].isnan().all() and same_outside(got, want, group=group)
+    for value in (float("inf"), -float("inf"), float("nan")):   # in a token's scale
+        bad = sa.clone()
+        bad[m - 1, 2] = value
+        got = gated(a, bad, w, sw, activation)
+        assert not got[1][m - 1].isfinite().any() and same_outside(got, want, rows=[m - 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("join", JOINS)
+def test_gated_product_of_zeros_and_of_groups_of_zeros(join):
+    m, n, k, a, sa, w, sw = gated_case(join, 71)
+    want = gated(a, sa, w, sw)
+    zero = a.clone()
+    zero.view(torch.uint8)[[0, m - 1]] = 0               # tokens of zeros
+    got = gated(zero, sa, w, sw)
+    assert (got[1][[0, m - 1]] == 1).all() and not (got[0][[0, m - 1]] & 0x7F).any()
+    assert same_outside(got, want, rows=[0, m - 1])
+    for first in (128, n + 128):                         # gate rows, or up rows, of the second group
+        last = min(first + 128, n if first < n else 2 * n)
+        zero = w.clone()
+        zero.view(torch.uint8)[first:last] = 0
+        got = gated(a, sa, zero, sw)
+        assert (got[1][:, 1] == 1).all() and not (got[0][:, 128:256] & 0x7F).any()
+        assert same_outside(got, want, group=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("join", JOINS)
+def test_gated_product_of_strided_operands(join):
+    """Rows inside wider matrices, scales stored column-major and inside wider ones."""
+    m, n, k, a, sa, w, sw = gated_case(join, 72)
+    want = gated(a, sa, w, sw)
+    # NaN bytes around the operands must not be read into the result
+    wa = torch.full((m, k + 112), 0x7F, dtype=torch.uint8, device=DEV)
+    ww = torch.full((2 * n, k + 48), 0x7F, dtype=torch.uint8, device=DEV)
+    wa[:, 16:16 + k], ww[:, 32:32 + k] = a.view(torch.uint8).to(DEV), w.view(torch.uint8).to(DEV)
+    sws = torch.full((2 * sw.size(0), 3 * sw.size(1)), float("nan"), device=DEV)
+    sws[::2, ::3] = sw.to(DEV)
+    got = gated(wa.view(F8)[:, 16:16 + k], sa.to(DEV).t().contiguous().t(), ww.view(F8)[:, 32:32 + k], sws[::2, ::3])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_gated_products_on_streams_that_overlap():
+    """Every join on every stream at once; the workspaces of the fp32 rows are a call's own."""
+    cases = [[t.to(DEV) for t in gated_case(join, 73)[3:]] for join in JOINS]
+    want = [dense.fp8_gemm_act_mul_quant(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(4 * len(cases)):
+        with torch.cuda.stream(streams[i % 4]):
+            at = (i + i // 4) % len(cases)
+            got.append((at, dense.fp8_gemm_act_mul_quant(*cases[at])))
+    torch.cuda.synchronize()
+    status_ok()
+    for at, (q, s) in got:
+        assert torch.equal(q.view(torch.uint8), want[at][0].view(torch.uint8)) and torch.equal(s, want[at][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [32768, 32784])
+def test_gated_product_beyond_32_bit_offsets(n):
+    """2.3 billion outputs, and for the second width as many pairs of fp32 rows: the rows at
+    both ends against the oracle, the zeros between."""
+    m, k = 70000, 144
+    a, sa, w, sw = gemm_case(64, 2 * n, k, 74)
+    sa = sa * 0.03
+    big_a = torch.zeros(m, k, device=DEV).to(F8)
+    big_sa = torch.ones(m, 2, device=DEV)
+    at = torch.cat([torch.arange(0, 32), torch.arange(m - 32, m)])
+    big_a.view(torch.uint8)[at.to(DEV)] = a.view(torch.uint8).to(DEV)
+    big_sa[at.to(DEV)] = sa.to(DEV)
+    q, s = dense.fp8_gemm_act_mul_quant(big_a, big_sa, w.to(DEV), sw.to(DEV))
+    status_ok()
+    h, e = O.fp8_gemm(a, sa, w, sw), gemm_error(a, sa, w, sw)
+    err = 1.13 * e[:, :n] * (h[:, n:].abs() + e[:, n:]) + h[:, :n].abs() * e[:, n:]
+    check_rows(q[at.to(DEV)], s[at.to(DEV)], O.act_mul(h, "silu"), True, GATE_REL, err)
+    assert (s[32:m - 32] == 1).all()
+    for lo in range(32, m - 32, 9000):                   # a piece at a time: no second copy of it all
+        assert not (q[lo:min(lo + 9000, m - 32)].view(torch.uint8) & 0x7F).any()
 
 
 # -------------------------------------------------------------------- the build
