@@ -205,7 +205,10 @@ int strix_w8a8_int8_gemm(void* out, int32_t* acc_out, const void* a_q, const flo
  * 128), ceil(k / 128)], any element strides; out bf16 / fp16 / fp32 (out_kind 0 / 1
  * / 2) [m, n]; bias NULL or [n] in the output's type. k must be a multiple of 16
  * (the last block may be short), m and n are free. Sums and scales in fp32, one
- * rounding at the end; no scratch, and the result does not depend on timing. The
+ * rounding at the end; no scratch, and the result does not depend on timing. The two
+ * scales are multiplied first, and subnormal fp32 numbers count as zero: a block whose
+ * a_scale * w_scale is below 2^-126 adds nothing, one whose product passes 2^128 gives an
+ * infinity or a NaN, whatever its sum. out must not overlap an input. The
  * reference has this weight format with 16-bit activations only
  * (csrc/gemm/fp8_wmma_gemm.hip, schema csrc/torch_ops.cpp:256). tcgen05
  * kind::f8f6f4; a launch may follow its predecessor's start (programmatic
@@ -241,9 +244,15 @@ int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, const float* a
  * (row, 128 columns), k a multiple of 16. fp8 == 0: q int8 [rows, k], scales fp32
  * [rows] (s_stride apart) = amax / 127, k a multiple of 8. A scale below the smallest
  * normal number (an all-zero group) is 1; q = y / scale to nearest even; a NaN or an
- * infinity in a group shows in its scale. x, residual bf16 (fp16 if in_f16), weight
- * of the same type or fp32 (weight_f32); element strides (of a single row they are not
- * read), rows on 16-byte boundaries, k at most 65,536. vLLM's norm does this step in the reference's deployment, in
+ * infinity in a group shows in its scale. Scales and quotients are products with
+ * reciprocals, each within three fp32 steps of the formula's, so a value as close as
+ * that to a border between two 8-bit values may fall to either side (one in a million
+ * does). Subnormal fp32 numbers count as zero. The squares are summed in fp32: where the
+ * sum passes 2^128 (bf16 rows with values beyond 1e19) the row comes out as zeros. x,
+ * residual bf16 (fp16 if in_f16), weight of the same type or fp32 (weight_f32); element
+ * strides (of a single row they are not read), rows on 16-byte boundaries, k at most
+ * 65,536. q and scales must not overlap an input. vLLM's norm does this step in the
+ * reference's deployment, in
  * 16 bits; its GEMMs quantise (csrc/gemm/w8a8_wmma_gemm.hip:508-529). */
 int strix_rms_norm_quant(const void* x, const void* residual, void* residual_out, const void* weight,
                          void* q, float* scales, int64_t rows, int64_t k, int64_t x_stride,

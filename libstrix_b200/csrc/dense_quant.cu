@@ -76,7 +76,9 @@ struct NormArgs {
 // Measured (bf16, residual): 4,096 x 5,120 23.5 us, 8,192 x 5,120 47 us = 6.2 TB/s (a CTA per row
 // without the row ahead: 34 and 63 us); one row of 5,120 2.3 us, a launch and its latency.
 // Two vectors per thread need 64 registers; four (rows beyond 16,384 columns) have none left
-// for the row ahead: 2,000 x 32,768 82 us = 5.6 TB/s.
+// for the row ahead: 2,000 x 32,768 82 us = 5.6 TB/s. Eight (beyond 32,768 columns) do not fit
+// 64 registers at all and spill about 500 bytes per thread: 2,000 x 32,784 157 us = 2.9 TB/s,
+// 1,000 x 65,536 140 us = 3.3.
 template <bool F8, bool F16, bool WF32, int V>
 __global__ void __launch_bounds__(kMaxRowThreads) rms_norm_quant_kernel(const NormArgs p) {
   pdl_enter();

@@ -74,7 +74,8 @@ def rms_norm_quant(x, weight, eps: float = 1e-6, residual=None, residual_out=Non
     receives x + residual rounded to x's dtype: a tensor of its own, or x or residual
     itself for an update in place. The norm is taken of the fp32 sum, before that
     rounding. q_dtype float8_e4m3fn: scales fp32 [M, ceil(K / 128)], K a multiple of 16;
-    int8: scales fp32 [M], K a multiple of 8."""
+    int8: scales fp32 [M], K a multiple of 8. Scales and quotients are within a few fp32
+    steps of amax / 448 (127) and y / scale."""
     fp8 = _is_fp8(q_dtype)
     if _eager(x, weight, residual, residual_out):
         return torch_ops._rms_norm_quant(x, weight, eps, residual, residual_out, fp8)
@@ -94,7 +95,8 @@ def act_mul_quant(x, activation: str = "silu", q_dtype=FP8):
 
 def fp8_gemm(a_q, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16):
     """[M, N] of a_q e4m3 [M, K] (a_scale fp32 [M, ceil(K / 128)]) and w e4m3 [N, K]
-    (w_scale fp32 [ceil(N / 128), ceil(K / 128)]), K a multiple of 16."""
+    (w_scale fp32 [ceil(N / 128), ceil(K / 128)]), K a multiple of 16. The two scales of a
+    block are multiplied first, in fp32: their product has to be a normal number."""
     ns = torch_ops if _eager(a_q, a_scale, w, w_scale, bias) else torch.ops.strix
     return ns.w8a8_fp8_gemm(a_q, a_scale, w, w_scale, bias, out_dtype)
 
