@@ -43,7 +43,7 @@ def apply_fp8_w8a8(x_2d: torch.Tensor, w: torch.Tensor, scales: torch.Tensor,
     bf16 is added to fp32 sums (to the 16-bit ones up to 8 rows); the result is bf16."""
     x_2d = x_2d.contiguous()
     own = bias is None or bias.dtype == torch.bfloat16
-    if x_2d.size(0) <= 8 and w.size(0) % 16 == 0:
+    if 0 < x_2d.size(0) <= 8 and w.size(0) % 16 == 0:   # (that kernel refuses an empty batch)
         out = apply_fp8(x_2d, w, scales, bias if own else None)
         return out if own else (out + bias).to(torch.bfloat16)
     from libstrix_b200 import dense, moe

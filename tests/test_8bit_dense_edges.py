@@ -155,7 +155,7 @@ def test_int8_mlp_blocks_chain_in_fp16():
 
 
 # ---------------------------------------------------------------- vLLM linear
-@pytest.mark.parametrize("rows", [3, 9])
+@pytest.mark.parametrize("rows", [0, 3, 9])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_vllm_linear_hands_the_kernels_a_bias_of_their_type(monkeypatch, rows, dtype):
     """With products that refuse what the kernels refuse, and add the bias as they do."""
@@ -168,7 +168,7 @@ def test_vllm_linear_hands_the_kernels_a_bias_of_their_type(monkeypatch, rows, d
         return out.to(out_dtype)
 
     def few(x, w, scales, bias):
-        assert bias is None or bias.dtype == torch.bfloat16
+        assert 1 <= x.size(0) <= 8 and (bias is None or bias.dtype == torch.bfloat16)
         return product(x, None, w, scales, bias, torch.bfloat16)
 
     monkeypatch.setattr(moe, "act_quant_fp8", lambda x: (x, None))
@@ -180,7 +180,7 @@ def test_vllm_linear_hands_the_kernels_a_bias_of_their_type(monkeypatch, rows, d
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [3, 9, 100])
+@pytest.mark.parametrize("rows", [0, 3, 9, 100])
 def test_vllm_linear_with_an_fp32_bias(rows):
     from strix_vllm import fp8
 
