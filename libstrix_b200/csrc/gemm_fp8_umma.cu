@@ -934,7 +934,8 @@ static bool gated_in_one(int64_t n) { return n % 128 == 0; }
 
 extern "C" int64_t strix_w8a8_fp8_gated_workspace(int64_t m, int64_t n, int64_t k) {
   if (m < 0 || n <= 0 || k <= 0 || m >= (int64_t(1) << 31) || n >= (int64_t(1) << 30)) return -1;
-  return gated_in_one(n) ? 0 : m * 2 * n * 4;
+  if (gated_in_one(n)) return 0;
+  return m <= INT64_MAX / (8 * n) ? m * 8 * n : -1;   // (m * 8 * n may pass 63 bits)
 }
 
 extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, const float* a_scale,
@@ -967,7 +968,8 @@ extern "C" int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, con
     const int splits = wide_plan(m, 2 * n, p.nkb, true, places).splits;
     return launch_wide<256, true>(p, splits, places[1], a_q, a_stride, w, w_stride, k, dev, st);
   }
-  const int64_t need = m * 2 * n * 4;
+  const int64_t need = strix_w8a8_fp8_gated_workspace(m, n, k);
+  STRIX_CHECK(need >= 0, "matrix too large");
   STRIX_CHECK(workspace_bytes >= need && workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
               "workspace must hold %lld bytes on a 16-byte boundary", (long long)need);
   p.out = workspace, p.out_kind = kOutF32, p.out_st = 2 * n;

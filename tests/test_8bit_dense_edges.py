@@ -11,7 +11,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from libstrix_b200 import dense, torch_ops
+from libstrix_b200 import _lib, dense, torch_ops
 from oracle import dense as O
 from test_8bit_dense_layer import DEV, F8, GATE_REL, check_rows, gemm_case, gemm_error, norm_case, status_ok
 
@@ -424,3 +424,13 @@ def test_kernel_sources_have_no_switches():
     found = [f"{f.name}:{i}" for f in sorted(csrc.iterdir()) for i, line in enumerate(f.read_text().splitlines(), 1)
              if re.match(r"\s*#\s*(if|ifdef|ifndef|elif)\b", line)]
     assert not found
+
+
+def test_gated_workspace_of_sizes_beyond_63_bits():
+    size = _lib.load().strix_w8a8_fp8_gated_workspace
+    m, n = (1 << 31) - 257, (1 << 30) - 144
+    assert m * 8 * n > 2 ** 63 and size(m, n, 16) == -1
+    assert size(m, (1 << 30) - 256, 16) == 0              # one kernel: no rows in between
+    m = 2 ** 63 // (8 * n)                                # the most that 63 bits hold
+    assert size(m, n, 16) == m * 8 * n and size(m + 1, n, 16) == -1
+    assert size(70000, 144, 16) == 70000 * 144 * 8
