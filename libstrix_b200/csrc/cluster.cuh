@@ -65,7 +65,8 @@ inline cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned size, un
   return cudaLaunchKernelEx(&cfg, kernel, P(static_cast<A&&>(args))...);
 }
 
-// How many clusters of `size` CTAs the current device runs at once, at one CTA per SM.
+// How many clusters of `size` CTAs the current device runs at once, at one CTA per SM. Two
+// threads may fill one table of answers at the same time: *out is written once, with the answer.
 template <typename... P>
 inline cudaError_t places(int* out, void (*kernel)(P...), unsigned size, unsigned block, size_t smem) {
   cudaLaunchConfig_t cfg{};
@@ -74,7 +75,10 @@ inline cudaError_t places(int* out, void (*kernel)(P...), unsigned size, unsigne
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = size, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cfg.attrs = &attr, cfg.numAttrs = 1;
-  return cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
+  int n = 0;
+  const cudaError_t err = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  if (err == cudaSuccess) *out = n;
+  return err;
 }
 
 }  // namespace cluster

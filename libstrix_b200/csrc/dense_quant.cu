@@ -314,8 +314,11 @@ int device_sms(int& dev, int& sms) {
   static int count[64] = {};
   STRIX_CUDA(cudaGetDevice(&dev));
   STRIX_CHECK(dev >= 0 && dev < 64, "device index %d out of range", dev);
-  if (!count[dev]) STRIX_CUDA(cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev));
   sms = count[dev];
+  if (sms == 0) {
+    STRIX_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    count[dev] = sms;
+  }
   return STRIX_OK;
 }
 
@@ -337,8 +340,11 @@ int launch_norm_v(const NormArgs& p, int threads, int sms, int dev, cudaStream_t
   auto kernel = rms_norm_quant_kernel<F8, F16, WF32, V>;
   // CTAs of this size that an SM holds at once (asked once per device and size)
   static int resident[64][kMaxRowThreads / 32] = {};
-  int& per_sm = resident[dev][threads / 32 - 1];
-  if (per_sm == 0) STRIX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0));
+  int per_sm = resident[dev][threads / 32 - 1];
+  if (per_sm == 0) {
+    STRIX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0));
+    resident[dev][threads / 32 - 1] = per_sm;
+  }
   STRIX_CHECK(per_sm > 0, "rms_norm_quant does not fit the device");
   const int64_t slots = int64_t(sms) * per_sm;
   launch_chain(kernel, unsigned(p.rows < slots ? p.rows : slots), threads, 0, st, p);

@@ -434,3 +434,39 @@ def test_gated_workspace_of_sizes_beyond_63_bits():
     m = 2 ** 63 // (8 * n)                                # the most that 63 bits hold
     assert size(m, n, 16) == m * 8 * n and size(m + 1, n, 16) == -1
     assert size(70000, 144, 16) == 70000 * 144 * 8
+
+
+@pytest.mark.gpu
+def test_first_calls_from_many_threads():
+    """A C call gives up the interpreter's lock, so the first calls of a process may meet in
+    the tables that they fill."""
+    import subprocess
+    import sys
+
+    code = """
+import threading, torch
+from libstrix_b200 import dense
+f8 = torch.float8_e4m3fn
+torch.manual_seed(0)
+x = torch.randn(300, 2048, device="cuda").bfloat16()
+nw = torch.ones(2048, device="cuda").bfloat16()
+w13, w2 = torch.randn(1024, 2048, device="cuda").to(f8), torch.randn(2048, 512, device="cuda").to(f8)
+s13, s2 = torch.rand(8, 16, device="cuda"), torch.rand(16, 4, device="cuda")
+rows = (3, 20, 50, 300)
+out, gate = [None] * 16, threading.Barrier(16)
+torch.cuda.synchronize()
+
+def work(i):
+    stream = torch.cuda.Stream()
+    gate.wait()
+    with torch.cuda.stream(stream):
+        out[i] = dense.fused_mlp_fp8_w8a8(x[:rows[i % 4]], nw, w13, s13, w2, s2)
+    stream.synchronize()
+
+threads = [threading.Thread(target=work, args=(i,)) for i in range(16)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+for i in range(16):
+    assert torch.equal(out[i], dense.fused_mlp_fp8_w8a8(x[:rows[i % 4]], nw, w13, s13, w2, s2)), i
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=240, cwd=Path(__file__).resolve().parent.parent)
