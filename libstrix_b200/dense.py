@@ -12,8 +12,10 @@ python/strix_vllm/fp8.py:121-262), with vLLM's 16-bit norm and silu_and_mul betw
 from __future__ import annotations
 
 import torch
+from torch import Tensor, is_grad_enabled
 from torch.autograd import forward_ad
 from torch.compiler import is_compiling
+from torch.nn import Parameter
 
 from . import torch_ops
 
@@ -32,22 +34,19 @@ def _plain(*tensors) -> bool:
     dispatcher attaches a node that warns in the backward pass, and a forward-mode tangent
     would be lost without a word there too, so it is refused here."""
     if (_are_functorch_transforms_active is None or _are_functorch_transforms_active()
-            or _len_torch_dispatch_stack() != 0 or _is_tracing()):
+            or _len_torch_dispatch_stack() or _is_tracing()):
         return False
-    grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is None:
-            continue
-        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter or grad and t.requires_grad:
+        if t is not None and (type(t) is not Tensor and type(t) is not Parameter
+                              or t.requires_grad and is_grad_enabled()):
             return False
     return True
 
 
-def _no_tangents(*tensors) -> None:
-    if getattr(forward_ad, "_current_level", 0) >= 0:   # a dual level is open
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError("the 8-bit dense layer has no forward-mode derivative")
+def _refuse_tangents(*tensors) -> None:
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the 8-bit dense layer has no forward-mode derivative")
 
 
 def _eager(first, *others) -> bool:
@@ -57,7 +56,8 @@ def _eager(first, *others) -> bool:
     Anything else takes torch.ops.strix, with its shape inference and errors."""
     if is_compiling():
         return False
-    _no_tangents(first, *others)
+    if getattr(forward_ad, "_current_level", 0) >= 0:   # a dual level is open
+        _refuse_tangents(first, *others)
     return first.is_cuda and _plain(first, *others)
 
 
