@@ -225,8 +225,9 @@ int strix_w8a8_fp8_gemm(void* out, const void* a_q, const float* a_scale, const 
  * halves, y = act(G) * U (gate_act 1 silu, 2 gelu_tanh) is quantised as
  * strix_act_mul_quant does: q e4m3 [m, n], scales fp32 [m, ceil(n / 128)]. n and k
  * multiples of 16. workspace: strix_w8a8_fp8_gated_workspace(m, n, k) bytes on a
- * 16-byte boundary (0: none needed, NULL allowed; -1: sizes no call takes), free again when the launches
- * have ended. Launches that may run at the same time need workspaces of their own. */
+ * 16-byte boundary (0: none needed, NULL allowed; -1: sizes that no call takes), free
+ * again when the launches have ended. Launches that may run at the same time need
+ * workspaces of their own. */
 int64_t strix_w8a8_fp8_gated_workspace(int64_t m, int64_t n, int64_t k);
 int strix_w8a8_fp8_gated(void* q, float* scales, const void* a_q, const float* a_scale, const void* w,
                          const float* w_scale, void* workspace, int64_t workspace_bytes, int64_t m,

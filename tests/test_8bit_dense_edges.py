@@ -470,3 +470,37 @@ for i in range(16):
     assert torch.equal(out[i], dense.fused_mlp_fp8_w8a8(x[:rows[i % 4]], nw, w13, s13, w2, s2)), i
 """
     subprocess.run([sys.executable, "-c", code], check=True, timeout=240, cwd=Path(__file__).resolve().parent.parent)
+
+
+# ------------------------------------------------- ends of the fp32 arithmetic
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_dtype", [F8, torch.int8])
+def test_norm_of_rows_whose_squares_leave_fp32(q_dtype):
+    """As the header says: zeros, and the other rows as they are."""
+    x, _, w = (t if t is None else t.to(DEV) for t in norm_case(3, 256, torch.bfloat16, 10, False))
+    want = dense.rms_norm_quant(x, w, q_dtype=q_dtype)
+    x[1] = 1e25
+    q, s = dense.rms_norm_quant(x, w, q_dtype=q_dtype)
+    assert not q[1].float().any() and (s[1] == 1).all()
+    assert torch.equal(q.view(torch.uint8)[::2], want[0].view(torch.uint8)[::2]) and torch.equal(s[::2], want[1][::2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [5, 100])
+def test_product_of_scales_that_leave_fp32(m):
+    """As the header says: the two scales are multiplied first. Below 2^-126 a block adds
+    nothing, beyond 2^128 it is not finite; up to those ends it is exact."""
+    n, k = 128, 256
+    a = torch.ones(m, k, device=DEV).to(F8)
+    w = torch.ones(n, k, device=DEV).to(F8)
+    sa, sw = torch.ones(m, 2, device=DEV), torch.ones(1, 2, device=DEV)
+
+    def first_block(x, y):
+        sa[:, 0], sw[:, 0] = x, y
+        return dense.fp8_gemm(a, sa, w, sw, out_dtype=torch.float32)
+
+    assert (first_block(2.0 ** -60, 2.0 ** -70) == 128).all()
+    assert not first_block(2.0 ** 70, 2.0 ** 60).isfinite().any()
+    sa[:, 1] = 0
+    assert (first_block(2.0 ** -60, 2.0 ** -66) == 128 * 2.0 ** -126).all()
+    assert (first_block(2.0 ** 60, 2.0 ** 60) == 128 * 2.0 ** 120).all()
